@@ -34,6 +34,7 @@ extern "C" {
 #define RL_ERR_COMPILE (-1002)     /* hiprtc rejected the program; see the build log */
 #define RL_ERR_IO (-1003)          /* code-object cache could not be read or written */
 #define RL_ERR_NO_DEVICE (-1004)   /* no usable HIP device */
+#define RL_ERR_INTERNAL (-1005)    /* something inside the library threw; see the text */
 
 typedef void* rl_module;
 typedef void* rl_function;
@@ -264,6 +265,80 @@ int rl_gemm_streamk_segments(const rl_gemm_config* cfg, int M, int N, int K, int
 /* One call for hosts that do not keep plans: plan_create (cached) + plan_launch. */
 int rl_gemm_f32(const rl_gemm_config* cfg, const float* A, const float* B, float* C, int M,
                 int N, int K, int lda, int ldb, int ldc, rl_stream stream);
+
+/* ---- products of a feed-forward block --------------------------------------------------------
+ * Not in the reference, which stops at one fp32 product (src/roller.py:62).  These run on kernels that are
+ * compiled with the library (no JIT at run time) and follow its conventions: status and text, device
+ * pointers, one device, NULL = the default stream, everything enqueued and nothing waited for.
+ * Matrices are row-major with a leading dimension in elements >= their columns; any alignment and any
+ * leading dimension is accepted, rows of whole aligned 16-byte chunks are fastest (others are copied into
+ * the workspace by the call, with more than 64 tokens).
+ *
+ * Workspace: the caller's (256-byte aligned, at least what the *_workspace_bytes function says; contents
+ * do not matter before or after; calls that share one must not overlap on the device), or NULL for one
+ * that the library keeps per stream (grown on demand, which waits for the stream; freed by
+ * rl_stream_destroy).  A call on a stream under capture needs the caller's: two graphs that may run at
+ * once need one each.  Inputs and outputs must not overlap, unless said otherwise. */
+
+#define RL_F32 0
+#define RL_F16 1
+#define RL_BF16 2
+
+#define RL_ACT_SILU 0      /* g / (1 + exp(-g)) */
+#define RL_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2 */
+#define RL_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+
+/* Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) Wd^T, for T rows (tokens) of x.
+ *   x[T, d_model], w_gate[d_ff, d_model], w_up[d_ff, d_model], w_down[d_model, d_ff], y[T, d_model],
+ * all of type dtype: weights as [outputs, inputs], the layout of trans_b above.  Products accumulate in
+ * fp32; act(g) * u is rounded once to dtype for the second product. */
+typedef struct rl_ffn_config {
+  int dtype;      /* RL_F32, RL_F16, RL_BF16 */
+  int activation; /* RL_ACT_* */
+  int d_model, d_ff;
+} rl_ffn_config;
+
+/* Workspace of a forward call of T tokens, and with `backward` the larger of that and a backward call's.
+ * `unaligned`: room for packed copies although d_model and d_ff are whole 16-byte chunks (pointers or
+ * leading dimensions that are not). */
+int rl_ffn_workspace_bytes(const rl_ffn_config* cfg, int T, int backward, int unaligned, size_t* bytes);
+
+/* Size of what a forward call keeps for the backward pass: x Wg^T and x Wu^T in fp32, their gated product
+ * in dtype. */
+int rl_ffn_saved_bytes(const rl_ffn_config* cfg, int T, size_t* bytes);
+
+/* `saved` (256-byte aligned, rl_ffn_saved_bytes) may be NULL: nothing is kept.  T == 0 is a no-op. */
+int rl_ffn_forward(const rl_ffn_config* cfg, const void* x, int ldx, const void* w_gate, int ld_gate, const void* w_up,
+                   int ld_up, const void* w_down, int ld_down, void* y, int ldy, int T, void* saved, void* workspace,
+                   size_t workspace_bytes, rl_stream stream);
+
+/* Gradients of sum(dy * y) for the inputs of a forward call that kept `saved`: dx[T, d_model] and the
+ * weights' gradients in the layout and type of the weights, overwritten.  dx may be NULL, dw_down may be
+ * NULL, dw_gate and dw_up may both be NULL: not computed.  `saved` is left as it was.  T == 0 writes zeros
+ * to the weights' gradients. */
+int rl_ffn_backward(const rl_ffn_config* cfg, const void* dy, int lddy, const void* x, int ldx, const void* w_gate,
+                    int ld_gate, const void* w_up, int ld_up, const void* w_down, int ld_down, const void* saved, void* dx,
+                    int lddx, void* dw_gate, int ldd_gate, void* dw_up, int ldd_up, void* dw_down, int ldd_down, int T,
+                    void* workspace, size_t workspace_bytes, rl_stream stream);
+
+/* Orthogonalises a matrix, or each of a stack of `batch`, by Newton-Schulz products (the update of the Muon
+ * optimiser): X = G / (||G||_F + eps); steps times X <- a X + (b A + c A A) X with A = X X^T (of the
+ * shorter side); O = scale * X.  G[rows, cols] and O[rows, cols] are of type dtype; O may be G. */
+typedef struct rl_ortho_config {
+  int dtype;      /* RL_F32, RL_F16, RL_BF16 */
+  int rows, cols, batch;
+  int steps;      /* 0 to 64 */
+  float eps, scale;
+} rl_ortho_config;
+
+int rl_ortho_workspace_bytes(const rl_ortho_config* cfg, size_t* bytes);
+
+/* `coefficients`: host memory, (a, b, c) for each step, read before the call returns; NULL: 3.4445, -4.7750,
+ * 2.0315 in every step.  They must keep |X| below 200 for bf16 matrices (operands are fp16 inside; any
+ * schedule that converges stays below 2).  stride_g, stride_o: elements from one matrix of the stack to
+ * the next. */
+int rl_orthogonalize(const rl_ortho_config* cfg, const float* coefficients, const void* G, int ldg, long stride_g, void* O,
+                     int ldo, long stride_o, void* workspace, size_t workspace_bytes, rl_stream stream);
 
 #ifdef __cplusplus
 }

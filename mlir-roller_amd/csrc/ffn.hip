@@ -1,0 +1,262 @@
+// The gated feed-forward block, for one element type (FFN_TYPE 0: fp32, 1: fp16, 2: bf16).
+//
+//   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T                        x[T,D], Wg[F,D], Wu[F,D], Wd[D,F]
+//   dh = dy Wd, dg = dh u act'(g), du = dh act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Two products forward (gate and up share their operand x and come out of one kernel, which also makes h)
+// and four backward (dh with dg and du made on the accumulators; dx as one sum over both pairs; dWg and dWu
+// as the two batch entries of one launch; dWd).  h, dg and du are rounded once to the element type, since
+// the next product's matrix instructions read that type; everything else between the inputs and the outputs
+// is fp32, g and u included, which the forward pass keeps for the backward pass.
+//
+// With few tokens (up to 64) both forward products read the weights once and do little else; they take the
+// few_rows kernel instead of the tile engine.
+#include "product_launch.h"
+#include "roller_ffn.h"
+
+namespace {
+
+using namespace product;
+
+#if FFN_TYPE == 0
+typedef float T;
+#define FFN_TABLE rl_ffn_f32
+#elif FFN_TYPE == 1
+typedef half_t T;
+#define FFN_TABLE rl_ffn_f16
+#else
+typedef bf16_t T;
+#define FFN_TABLE rl_ffn_bf16
+#endif
+
+constexpr int ES = sizeof(T), PER = 16 / ES;
+constexpr int FEW = 64;   // tokens up to which the forward products take the few_rows kernel
+constexpr int SPLIT_TOKENS = ES == 2 ? 16 : 0;   // tokens up to which h goes into the second product unrounded
+
+int pitch_of(int n) { return (n + PER - 1) / PER * PER; }
+
+// The tile engine reads whole 16-byte chunks: a matrix whose rows are anything else is packed first.
+bool aligned(const FfnMatrix& m, int cols) { return (uintptr_t)m.p % 16 == 0 && m.ld % PER == 0 && cols % PER == 0; }
+
+class Carver {
+ public:
+  explicit Carver(char* base) : base_(base) {}
+  char* take(size_t bytes) {
+    char* p = base_ ? base_ + used_ : nullptr;
+    used_ += ffn_round(bytes);
+    return p;
+  }
+  size_t used() const { return used_; }
+
+ private:
+  char* base_;
+  size_t used_ = 0;
+};
+
+// Space for a packed copy of m, if it needs one.
+T* pack_space(Carver& room, const FfnMatrix& m, int rows, int cols, bool need) {
+  (void)m;
+  return need ? (T*)room.take((size_t)rows * pitch_of(cols) * ES) : nullptr;
+}
+
+int pack(FfnMatrix& m, int rows, int cols, T* space, hipStream_t stream) {
+  if (!space) return RL_OK;
+  const int pitch = pitch_of(cols);
+  PT_TRY(launch(pack_kernel<T>, "packing an operand", dim3(blocks_for((long)rows * (pitch / PER))), 256, stream, (const T*)m.p, m.ld, rows, cols, space, pitch));
+  m = {space, pitch};
+  return RL_OK;
+}
+
+int vec_ok(const void* p, int ld) { return (uintptr_t)p % (4 * ES) == 0 && ld % 4 == 0; }
+
+Store<T> store(void* c, int ldc, int N) {
+  Store<T> s = {};
+  s.c[0] = s.c[1] = (T*)c;
+  s.ldc = s.ldc1 = ldc;
+  s.N = N;
+  s.vec = vec_ok(c, ldc);
+  return s;
+}
+
+Problem problem(const void* a, int lda, const void* b, int ldb, int M, int N, int K, int M_out, int N_out) {
+  Problem p = {};
+  p.a[0] = a;
+  p.b[0] = b;
+  p.lda = lda;
+  p.ldb = p.ldb1 = ldb;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.M_out = M_out;
+  p.N_out = N_out;
+  return p;
+}
+
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+
+// ---- forward ----
+
+struct ForwardRoom {
+  T *x, *w_gate, *w_up, *w_down, *h;
+  float* h32;
+  char* slabs;
+  size_t bytes;
+};
+
+ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
+  Carver room(c.room);
+  ForwardRoom r = {};
+  const FfnSaved s = ffn_saved(ES, c.T, c.F);
+  if (c.T <= SPLIT_TOKENS) r.h32 = (float*)room.take((size_t)c.T * s.pitch * 4);
+  else if (!c.saved) r.h = (T*)room.take((size_t)c.T * s.pitch * ES);
+  if (c.T > FEW) {
+    r.x = pack_space(room, c.x, c.T, c.D, unaligned || !aligned(c.x, c.D));
+    r.w_gate = pack_space(room, c.w_gate, c.F, c.D, unaligned || !aligned(c.w_gate, c.D));
+    r.w_up = pack_space(room, c.w_up, c.F, c.D, unaligned || !aligned(c.w_up, c.D));
+    r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
+    const size_t up = plan_product(ES, 1, 1, 0, c.T, s.pitch, c.D, 1, c.compute_units).slab_bytes;
+    const size_t down = plan_product(ES, 0, 1, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes;
+    r.slabs = room.take(larger(up, down));
+  }
+  r.bytes = room.used();
+  return r;
+}
+
+template <int BLOCKS, int SPLIT>
+int few_rows(const FfnCall& c, const void* h, const GatedForward<T>& gated, const Store<T>& out, int pitch) {
+  // Enough waves to keep the memory busy from every CU: up to 16 share the K of 16 weight rows, none with
+  // fewer than 256 bytes of each row.
+  auto waves = [&](int groups, int K) {
+    int w = 4;
+    while (w < 16 && (long)groups * w < 16L * c.compute_units && K * ES >= 512 * w) w *= 2;
+    return 64 * w;
+  };
+  typedef typename x_type<T, SPLIT>::type H;
+  const int up = (pitch + 15) / 16, down = (c.D + 15) / 16;
+  PT_TRY(launch(few_rows_kernel<T, BLOCKS, 1, 0, GatedForward<T>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
+                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, pitch, c.D, gated));
+  return launch(few_rows_kernel<T, BLOCKS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
+                c.D, c.D, c.F, out);
+}
+
+size_t forward_room(const FfnCall& c, bool unaligned) { return forward_carve(c, unaligned).bytes; }
+
+int forward(const FfnCall& call) {
+  FfnCall c = call;
+  const ForwardRoom r = forward_carve(c, false);
+  const FfnSaved s = ffn_saved(ES, c.T, c.F);
+  T* h = c.saved ? (T*)((char*)c.saved + s.h) : r.h;
+  GatedForward<T> gated = {};
+  gated.h = h;
+  gated.h32 = r.h32;
+  gated.g = c.saved ? (float*)((char*)c.saved + s.g) : nullptr;
+  gated.u = c.saved ? (float*)((char*)c.saved + s.u) : nullptr;
+  gated.pitch = s.pitch;
+  gated.kind = c.activation;
+  const Store<T> out = store(c.y, c.ldy, c.D);
+  if (c.T <= 16) return few_rows<1, SPLIT_TOKENS != 0>(c, r.h32 ? (const void*)r.h32 : h, gated, out, s.pitch);
+  if (c.T <= 32) return few_rows<2, 0>(c, h, gated, out, s.pitch);
+  if (c.T <= FEW) return few_rows<4, 0>(c, h, gated, out, s.pitch);
+
+  PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
+  PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
+  PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));
+  PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
+  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, s.pitch);
+  up.b[1] = c.w_up.p;
+  up.ldb1 = c.w_up.ld;
+  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: gate and up")));
+  const Problem down = problem(h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
+  return run_product<T, 1, 1, 0, 1, 0>(down, out, 1, r.slabs, c.stream, c.compute_units, "ffn: down");
+}
+
+// ---- backward ----
+
+struct BackwardRoom {
+  T *dy, *x, *w_gate, *w_up, *w_down, *dg, *du;
+  char* slabs;
+  size_t bytes;
+};
+
+BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
+  Carver room(c.room);
+  BackwardRoom r = {};
+  const FfnSaved s = ffn_saved(ES, c.T, c.F);
+  const size_t n = (size_t)c.T * s.pitch * ES;
+  // (dg and du directly behind each other: the two batch entries of one product)
+  r.dg = (T*)room.take(2 * n);
+  r.du = r.dg ? r.dg + (size_t)c.T * s.pitch : nullptr;
+  r.dy = pack_space(room, c.dy, c.T, c.D, unaligned || !aligned(c.dy, c.D));
+  r.x = pack_space(room, c.x, c.T, c.D, unaligned || !aligned(c.x, c.D));
+  // dx reads both weights with one leading dimension
+  const bool weights = unaligned || !aligned(c.w_gate, c.D) || !aligned(c.w_up, c.D) || c.w_gate.ld != c.w_up.ld;
+  r.w_gate = pack_space(room, c.w_gate, c.F, c.D, weights);
+  r.w_up = pack_space(room, c.w_up, c.F, c.D, weights);
+  r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
+  size_t slabs = plan_product(ES, 0, 1, 0, c.T, s.pitch, c.D, 1, c.compute_units).slab_bytes;
+  slabs = larger(slabs, plan_product(ES, 0, 2, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes);
+  slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.F, c.D, c.T, 2, c.compute_units).slab_bytes);
+  slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.D, c.F, c.T, 1, c.compute_units).slab_bytes);
+  r.slabs = room.take(slabs);
+  r.bytes = room.used();
+  return r;
+}
+
+size_t backward_room(const FfnCall& c, bool unaligned) { return backward_carve(c, unaligned).bytes; }
+
+int zero(void* p, int ld, int rows, int cols, hipStream_t stream) {
+  return launch(zero_kernel<T>, "ffn: zero gradient", dim3(blocks_for((long)rows * cols)), 256, stream, (T*)p, ld, rows, cols);
+}
+
+int backward(const FfnCall& call) {
+  FfnCall c = call;
+  if (c.T == 0) {   // no tokens: the gradients of the weights are zero
+    if (c.dw_gate) PT_TRY(zero(c.dw_gate, c.ld_dw_gate, c.F, c.D, c.stream));
+    if (c.dw_up) PT_TRY(zero(c.dw_up, c.ld_dw_up, c.F, c.D, c.stream));
+    if (c.dw_down) PT_TRY(zero(c.dw_down, c.ld_dw_down, c.D, c.F, c.stream));
+    return RL_OK;
+  }
+  const BackwardRoom r = backward_carve(c, false);
+  const FfnSaved s = ffn_saved(ES, c.T, c.F);
+  const T* h = (const T*)((char*)c.saved + s.h);
+  PT_TRY(pack(c.dy, c.T, c.D, r.dy, c.stream));
+  if (c.dw_down) {
+    const Problem p = problem(c.dy.p, c.dy.ld, h, s.pitch, c.D, c.F, c.T, c.D, c.F);
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, store(c.dw_down, c.ld_dw_down, c.F), 1, r.slabs, c.stream, c.compute_units, "ffn: dw_down")));
+  }
+  if (!c.dx && !c.dw_gate) return RL_OK;
+  PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
+  GatedBackward<T> gated = {};
+  gated.g = (const float*)((char*)c.saved + s.g);
+  gated.u = (const float*)((char*)c.saved + s.u);
+  gated.dg = r.dg;
+  gated.du = r.du;
+  gated.pitch = s.pitch;
+  gated.kind = c.activation;
+  const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, s.pitch);
+  PT_TRY((run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: dh")));
+  if (c.dx) {
+    PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
+    PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));
+    Problem p = problem(r.dg, s.pitch, c.w_gate.p, c.w_gate.ld, c.T, c.D, c.F, c.T, c.D);
+    p.a[1] = r.du;
+    p.b[1] = c.w_up.p;
+    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, store(c.dx, c.ld_dx, c.D), 1, r.slabs, c.stream, c.compute_units, "ffn: dx")));
+  }
+  if (c.dw_gate) {
+    PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
+    Problem p = problem(r.dg, s.pitch, c.x.p, c.x.ld, c.F, c.D, c.T, c.F, c.D);
+    p.batch_a = (long)c.T * s.pitch;
+    Store<T> out = store(c.dw_gate, c.ld_dw_gate, c.D);
+    out.c[1] = (T*)c.dw_up;
+    out.ldc1 = c.ld_dw_up;
+    out.vec = out.vec && vec_ok(c.dw_up, c.ld_dw_up);
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, out, 2, r.slabs, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
+  }
+  return RL_OK;
+}
+
+}  // namespace
+
+FfnType FFN_TABLE() { return {forward_room, backward_room, forward, backward}; }

@@ -1,0 +1,329 @@
+// What follows a product: the epilogues of the matrix-product engine (product_tile.h) for the gated
+// feed-forward block and for Newton-Schulz orthogonalisation, and the small kernels around them.
+//
+// An epilogue is a struct with at(batch, split), which picks the buffers of a batch entry, and
+// put(m, n, v): four consecutive columns n .. n+3 of row m, n a multiple of 4 (gated products:
+// put(m, n, gate, up)).
+
+#ifndef PRODUCT_OPS_H
+#define PRODUCT_OPS_H
+
+#include "product_tile.h"
+
+namespace product {
+
+template <class T>
+struct vec4;
+template <> struct vec4<float> { typedef v4f type; };
+template <> struct vec4<half_t> { typedef _Float16 type __attribute__((ext_vector_type(4))); };
+template <> struct vec4<bf16_t> { typedef __bf16 type __attribute__((ext_vector_type(4))); };
+
+// One rounding, to nearest even, from fp32 to the stored type.
+template <class T>
+PT_DEV typename vec4<T>::type round4(v4f v) {
+  typename vec4<T>::type o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (T)v[e];
+  return o;
+}
+
+// Internal buffers: pitch a multiple of 4 elements, 16-byte aligned.
+template <class T>
+PT_DEV void store4(T* at, v4f v) { *(typename vec4<T>::type*)at = round4<T>(v); }
+template <class T>
+PT_DEV v4f load4(const T* at) {
+  const typename vec4<T>::type x = *(const typename vec4<T>::type*)at;
+  return v4f{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+}
+
+// ---- activations ------------------------------------------------------------------------------------
+// Kept in fp32 throughout.  1 / (1 + 2^(-z log2 e)) from the exponential and the reciprocal of the
+// hardware, 1 ulp each: the ends are exact (0 and 1), NaN stays NaN.
+
+enum { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2 };
+
+PT_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
+
+constexpr float GELU_2C = 1.5957691216f, GELU_C1 = 0.044715f;   // 2 sqrt(2 / pi)
+
+PT_DEV float act(int kind, float g) {
+  if (kind == ACT_SILU) return g * sigmoid(g);
+  if (kind == ACT_GELU) return 0.5f * g * (1.0f + erff(0.70710678f * g));
+  return g * sigmoid(GELU_2C * (g + GELU_C1 * g * g * g));   // (1 + tanh z) / 2 = sigmoid(2 z)
+}
+
+// The activation and its slope.  The factors that grow with g stand beside ones that have long been zero
+// where they would overflow, so they are taken of g cut to +-32.
+PT_DEV void act_slope(int kind, float g, float& a, float& slope) {
+  const float c = fminf(fmaxf(g, -32.0f), 32.0f);
+  if (kind == ACT_SILU) {
+    const float s = sigmoid(g);
+    a = g * s;
+    slope = s * (1.0f + c * (1.0f - s));
+  } else if (kind == ACT_GELU) {
+    const float s = 0.5f * (1.0f + erff(0.70710678f * g));
+    a = g * s;
+    slope = s + c * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * c * c);
+  } else {
+    const float s = sigmoid(GELU_2C * (g + GELU_C1 * g * g * g));
+    a = g * s;
+    slope = s + c * s * (1.0f - s) * GELU_2C * (1.0f + 3.0f * GELU_C1 * c * c);
+  }
+}
+
+// ---- epilogues --------------------------------------------------------------------------------------
+
+// C = acc, in a caller's matrix: any leading dimension and alignment.
+template <class T>
+struct Store {
+  T* c[2];      // one per batch entry
+  int ldc, ldc1, N;
+  int vec;      // rows of 4 elements are aligned
+  __device__ __forceinline__ Store at(int batch, int) const {
+    Store o = *this;
+    if (batch) {
+      o.c[0] = c[1];
+      o.ldc = ldc1;
+    }
+    return o;
+  }
+  __device__ __forceinline__ void put(int m, int n, v4f v) const {
+    T* to = c[0] + (long)m * ldc + n;
+    if (vec && n + 3 < N) {
+      store4(to, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < N) to[e] = (T)v[e];
+    }
+  }
+};
+
+// h = act(g) u; for a later backward pass g and u as well, unrounded (a gradient made of g and u rounded
+// to 16 bits would carry two or three roundings where it now carries its own).
+template <class T>
+struct GatedForward {
+  T* h;           // NULL: only h32
+  float* h32;     // h unrounded, NULL: not needed
+  float *g, *u;   // NULL: not kept
+  int pitch, kind;
+  __device__ __forceinline__ GatedForward at(int, int) const { return *this; }
+  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up) const {
+    const long i = (long)m * pitch + n;
+    v4f o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = act(kind, gate[e]) * up[e];
+    if (h) store4(h + i, o);
+    if (h32) *(v4f*)(h32 + i) = o;
+    if (g) {
+      *(v4f*)(g + i) = gate;
+      *(v4f*)(u + i) = up;
+    }
+  }
+};
+
+// From dh: dg = dh u act'(g), du = dh act(g).
+template <class T>
+struct GatedBackward {
+  const float *g, *u;
+  T *dg, *du;
+  int pitch, kind;
+  __device__ __forceinline__ GatedBackward at(int, int) const { return *this; }
+  __device__ __forceinline__ void put(int m, int n, v4f dh) const {
+    const long i = (long)m * pitch + n;
+    const v4f gate = *(const v4f*)(g + i), up = *(const v4f*)(u + i);
+    v4f x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a, slope;
+      act_slope(kind, gate[e], a, slope);
+      x[e] = dh[e] * up[e] * slope;
+      y[e] = dh[e] * a;
+    }
+    store4(dg + i, x);
+    store4(du + i, y);
+  }
+};
+
+// ---- small kernels ----------------------------------------------------------------------------------
+
+// Sums the slabs of a split product in split order and hands them to the epilogue.
+template <class Epi, bool TWO>
+__global__ __launch_bounds__(256) void join_kernel(const Partial part, int splits, int tile, int M_out, int N_out, const Epi epi) {
+  const int quads = (N_out + 3) / 4;
+  const auto out = epi.at(blockIdx.z, 0);
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)M_out * quads; i += gridDim.x * 256L) {
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    if (tile && n / tile > m / tile) continue;   // (a symmetric product has no tiles above its diagonal)
+    const float* p = part.slab + (long)blockIdx.z * part.slab_size + (long)m * part.pitch + n;
+    v4f v = *(const v4f*)p, w = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (TWO) w = *(const v4f*)(p + part.slab_size);
+    for (int s = 1; s < splits; ++s) {
+      p += part.per_split * part.slab_size;
+      v += *(const v4f*)p;
+      if constexpr (TWO) w += *(const v4f*)(p + part.slab_size);
+    }
+    if constexpr (TWO) out.put(m, n, v, w);
+    else out.put(m, n, v);
+  }
+}
+
+// Copies a matrix whose rows are not whole aligned 16-byte chunks into one whose rows are, with zeros
+// behind each row's end.  One element per access: such rows may start at any address.
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* src, int ld, int rows, int cols, T* dst, int pitch) {
+  constexpr int PER = 16 / sizeof(T);
+  typedef T chunk __attribute__((ext_vector_type(PER)));
+  const int chunks = pitch / PER;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * chunks; i += gridDim.x * 256L) {
+    const int r = (int)(i / chunks), c = (int)(i % chunks) * PER;
+    chunk v;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] = c + e < cols ? src[(long)r * ld + c + e] : (T)0.0f;
+    *(chunk*)(dst + (long)r * pitch + c) = v;
+  }
+}
+
+// rows x cols zeros (the gradient of a weight over no tokens).
+template <class T>
+__global__ __launch_bounds__(256) void zero_kernel(T* c, int ld, int rows, int cols) {
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * cols; i += gridDim.x * 256L) c[i / cols * ld + i % cols] = (T)0.0f;
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------
+// A product with at most 16 * BLOCKS rows of x, bound by reading the weights once.  A workgroup owns 16
+// weight rows (GATED: 16 gate rows and the same 16 up rows) and its waves share out K, 128 bytes of each
+// row at a time; weights go from memory straight into the MFMA's registers (row lane % 16, 16-byte chunk
+// lane / 16 of each 64 bytes), many loads in flight per wave, no LDS until the waves' sums are added up.
+// Rows of x and of the weights may start at any element: a chunk is loaded whole, at the alignment of
+// its type, and the last one of a row element by element.
+template <class T>
+PT_DEV v4u whole_chunk(const T* at) {
+  v4u v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(at, sizeof(T)), 16);
+  return v;
+}
+template <class T>
+PT_DEV v4u chunk_at(const T* row, int k, int K) {
+  constexpr int PER = 16 / sizeof(T);
+  if (k + PER <= K) return whole_chunk(row + k);
+  typedef T chunk __attribute__((ext_vector_type(PER)));
+  chunk v;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) v[e] = k + e < K ? row[k + e] : (T)0.0f;
+  return __builtin_bit_cast(v4u, v);
+}
+
+//
+// SPLIT: x is fp32 although the weights have 16 bits.  Each of its elements then goes into the product as
+// the sum of two of 16 bits, high part and remainder: twice the matrix instructions, which are idle anyway,
+// and no rounding of x that the result could show.
+template <class T, int SPLIT>
+struct x_type { typedef T type; };
+template <class T>
+struct x_type<T, 1> { typedef float type; };
+
+template <class T>
+PT_DEV void split_chunk(const float* x, v4u& hi, v4u& lo) {
+  typedef T chunk __attribute__((ext_vector_type(8)));
+  chunk h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    h[e] = (T)x[e];
+    l[e] = (T)(x[e] - (float)h[e]);
+  }
+  hi = __builtin_bit_cast(v4u, h);
+  lo = __builtin_bit_cast(v4u, l);
+}
+
+template <class T, int BLOCKS, int GATED, int SPLIT, class Epi>
+__global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T, SPLIT>::type* x, int ldx, const T* w0, int ldw0, const T* w1, int ldw1, int M, int N, int N_out, int K, const Epi epi) {
+  constexpr int PER = 16 / sizeof(T), W = GATED ? 2 : 1, UNROLL = BLOCKS == 1 ? 8 : BLOCKS == 2 ? 4 : 2;
+  const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int n0 = blockIdx.x * 16, row = n0 + lr < N ? n0 + lr : N - 1;   // (a row past the end is not stored)
+  const T* wr[2] = {w0 + (long)row * ldw0, GATED ? w1 + (long)row * ldw1 : nullptr};
+  typedef typename x_type<T, SPLIT>::type X;
+  const X* xr[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) xr[b] = x + (long)(16 * b + lr < M ? 16 * b + lr : M - 1) * ldx;
+
+  v4f acc[W][BLOCKS];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) acc[w][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // the waves take turns at groups of UNROLL x 64 bytes of k
+  constexpr int GROUP = UNROLL * 4 * PER, XV = SPLIT ? 2 : 1;   // XV: 16-byte loads per chunk of x
+  for (int k0 = wave * GROUP; k0 < K; k0 += waves * GROUP) {
+    v4u wv[W][UNROLL], xv[BLOCKS][UNROLL][XV];
+    const bool whole = k0 + GROUP <= K;
+#pragma unroll
+    for (int t = 0; t < UNROLL; ++t) {
+      const int k = k0 + (t * 4 + lg) * PER;
+#pragma unroll
+      for (int w = 0; w < W; ++w) wv[w][t] = whole ? whole_chunk(wr[w] + k) : chunk_at(wr[w], k, K);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int v = 0; v < XV; ++v) xv[b][t][v] = whole ? whole_chunk(xr[b] + k + 4 * v) : chunk_at(xr[b], k + 4 * v, K);
+    }
+#pragma unroll
+    for (int t = 0; t < UNROLL; ++t)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        v4u hi = xv[b][t][0], lo;
+        if constexpr (SPLIT) {
+          float f[8];
+          __builtin_memcpy(f, &xv[b][t][0], 16);
+          __builtin_memcpy(f + 4, &xv[b][t][XV - 1], 16);
+          split_chunk<T>(f, hi, lo);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          acc[w][b] = mma<T, 16>::run(wv[w][t], hi, acc[w][b]);
+          if constexpr (SPLIT) acc[w][b] = mma<T, 16>::run(wv[w][t], lo, acc[w][b]);
+        }
+      }
+  }
+
+  // the waves' sums, added in wave order
+  __shared__ v4f sums[16 * 64];
+  const auto out = epi.at(0, 0);
+  v4f total[W][BLOCKS];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      __syncthreads();
+      sums[wave * 64 + lane] = acc[w][b];
+      __syncthreads();
+      if (wave == 0) {
+        v4f v = sums[lane];
+        for (int s = 1; s < waves; ++s) v += sums[s * 64 + lane];
+        total[w][b] = v;
+      }
+    }
+  if (wave != 0) return;
+  const int n = n0 + 4 * lg;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const int m = 16 * b + lr;
+    if (m >= M || n >= N_out) continue;
+    // columns past the last weight row: zeros (padding of h), or not stored
+    if constexpr (GATED) {
+      v4f g = total[0][b], u = total[W - 1][b];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e >= N) g[e] = u[e] = 0.0f;
+      out.put(m, n, g, u);
+    } else {
+      out.put(m, n, total[0][b]);
+    }
+  }
+}
+
+}  // namespace product
+
+#endif

@@ -7,6 +7,7 @@
 // .incbin and handed to hiprtc at run time.
 
 #include "roller_hip.h"
+#include "roller_internal.h"
 #include "roller_scratch.h"
 
 #include <hip/hip_runtime_api.h>
@@ -594,6 +595,27 @@ int launch_plan(const rl_gemm_plan* plan, const float* A, const float* B, float*
 
 }  // namespace
 
+// ---- for the other translation units of the library (roller_internal.h) ----
+
+int rl_fail(int code, const char* fmt, ...) {
+  char buf[2048];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  g_error = buf;
+  return code;
+}
+
+int rl_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+
+int rl_device(int* device, int* compute_units) {
+  if (!g_ready) return fail(RL_ERR_NO_DEVICE, "rl_init has not been called (or failed)");
+  *device = g_device.load();
+  *compute_units = g_compute_units.load();
+  return RL_OK;
+}
+
 extern "C" {
 
 int rl_init(int device) {
@@ -792,6 +814,8 @@ int rl_stream_destroy(rl_stream s) {
       g_workspaces.erase(it);
     }
   }
+  int rc = rl_products_forget_stream((hipStream_t)s);
+  if (rc) return rc;
   HIP_TRY(hipStreamDestroy((hipStream_t)s));
   return RL_OK;
 }

@@ -33,6 +33,7 @@ RL_ERR_INVALID_ARG = -1001
 RL_ERR_COMPILE = -1002
 RL_ERR_IO = -1003
 RL_ERR_NO_DEVICE = -1004
+RL_ERR_INTERNAL = -1005
 
 
 class HipError(RuntimeError):
@@ -63,6 +64,16 @@ class _GemmConfigC(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "bm", "bn", "bk", "wm", "wn", "mi", "stages", "pad_a", "pad_b", "vec", "edge", "swz",
         "group", "accum", "direct", "trans_b", "streamk")]
+
+
+class FfnConfig(C.Structure):
+    """``rl_ffn_config``: one gated feed-forward block."""
+    _fields_ = [(n, C.c_int) for n in ("dtype", "activation", "d_model", "d_ff")]
+
+
+class OrthoConfig(C.Structure):
+    """``rl_ortho_config``: a stack of matrices to orthogonalise."""
+    _fields_ = [(n, C.c_int) for n in ("dtype", "rows", "cols", "batch", "steps")] + [("eps", C.c_float), ("scale", C.c_float)]
 
 
 class StreamKSchedule(C.Structure):
@@ -129,28 +140,41 @@ class GemmConfig:
 # building and loading the shared library
 # --------------------------------------------------------------------------------------------
 
+HIPCC_LIBRARY_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def build_library(verbose: bool = False) -> Path:
-    """Builds libroller_hip.so: csrc/roller_hip.cpp (host code; the kernel template is embedded as text
-    and compiled for gfx950 by hiprtc at run time or by ``precompile``) and csrc/roller_scratch.hip
-    (hipcc, gfx950: the static scratch array of the launch entry point that allocates nothing)."""
+    """Builds libroller_hip.so: csrc/roller_hip.cpp (host code; the GEMM template is embedded as text
+    and compiled for gfx950 by hiprtc at run time or by ``precompile``), csrc/roller_scratch.hip
+    (hipcc, gfx950: the static scratch array of the launch entry point that allocates nothing), and the
+    products of a feed-forward block, a closed set of kernels that is compiled here (csrc/ffn.hip once per
+    element type, csrc/orthogonalize.hip) behind csrc/roller_products.cpp."""
+    import concurrent.futures as cf
+
     template = CSRC_DIR / "gemm_f32_mfma.hip"
     obj_dir = REPO_ROOT / "build"
     obj_dir.mkdir(exist_ok=True)
-    scratch_obj = obj_dir / "roller_scratch.o"
-    cmds = [
-        ["hipcc", "--offload-arch=gfx950", "-O2", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-         f"-I{CSRC_DIR}", "-c", str(CSRC_DIR / "roller_scratch.hip"), "-o", str(scratch_obj)],
-        ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
-         "-D__HIP_PLATFORM_AMD__", f"-I{ROCM / 'include'}", f"-I{REPO_ROOT / 'include'}",
-         f'-DRL_TEMPLATE_PATH="{template}"', f'-DRL_SK_DECODE_PATH="{CSRC_DIR / "gemm_sk_decode.inc"}"',
-         f"-I{CSRC_DIR}", str(CSRC_DIR / "roller_hip.cpp"), str(scratch_obj),
-         "-o", str(LIB_PATH), f"-L{ROCM / 'lib'}", "-lamdhip64", "-lhiprtc",
-         f"-Wl,-rpath,{ROCM / 'lib'}"],
-    ]
-    for cmd in cmds:
+    units = [("roller_scratch", "roller_scratch.hip", []), ("orthogonalize", "orthogonalize.hip", [])]
+    units += [(f"ffn_{name}", "ffn.hip", [f"-DFFN_TYPE={i}"]) for i, name in enumerate(("f32", "f16", "bf16"))]
+    include = [f"-I{CSRC_DIR}", f"-I{REPO_ROOT / 'include'}"]
+
+    def run(cmd):
         if verbose:
             print(" ".join(cmd))
-        subprocess.run(cmd, check=True)
+        done = subprocess.run(cmd, capture_output=True, text=True)
+        if done.returncode != 0:
+            raise RuntimeError(f"{' '.join(cmd)} failed:\n{done.stderr}")
+
+    objects = [str(obj_dir / f"{name}.o") for name, _, _ in units]
+    with cf.ThreadPoolExecutor(max_workers=8) as pool:
+        list(pool.map(run, [["hipcc", *HIPCC_LIBRARY_FLAGS, *include, *defines, "-c", str(CSRC_DIR / source), "-o", obj]
+                            for (_, source, defines), obj in zip(units, objects)]))
+    run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wextra",
+         "-D__HIP_PLATFORM_AMD__", f"-I{ROCM / 'include'}", *include,
+         f'-DRL_TEMPLATE_PATH="{template}"', f'-DRL_SK_DECODE_PATH="{CSRC_DIR / "gemm_sk_decode.inc"}"',
+         str(CSRC_DIR / "roller_hip.cpp"), str(CSRC_DIR / "roller_products.cpp"), *objects,
+         "-o", str(LIB_PATH), f"-L{ROCM / 'lib'}", "-lamdhip64", "-lhiprtc",
+         f"-Wl,-rpath,{ROCM / 'lib'}"])
     global _lib
     _lib = None
     return LIB_PATH
@@ -201,6 +225,14 @@ _SIGNATURES = {
     "rl_gemm_plan_launch_static": ([C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p] + [C.c_int] * 6 + [C.c_void_p], C.c_int),
     "rl_gemm_streamk_schedule": ([C.POINTER(_GemmConfigC)] + [C.c_int] * 4 + [C.POINTER(StreamKSchedule)], C.c_int),
     "rl_gemm_streamk_segments": ([C.POINTER(_GemmConfigC)] + [C.c_int] * 5 + [C.POINTER(StreamKSegment), C.c_int, C.POINTER(C.c_int)], C.c_int),
+    "rl_ffn_workspace_bytes": ([C.POINTER(FfnConfig), C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "rl_ffn_saved_bytes": ([C.POINTER(FfnConfig), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "rl_ffn_forward": ([C.POINTER(FfnConfig)] + [C.c_void_p, C.c_int] * 5 + [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
+    "rl_ffn_backward": ([C.POINTER(FfnConfig)] + [C.c_void_p, C.c_int] * 5 + [C.c_void_p] + [C.c_void_p, C.c_int] * 4
+                        + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
+    "rl_ortho_workspace_bytes": ([C.POINTER(OrthoConfig), C.POINTER(C.c_size_t)], C.c_int),
+    "rl_orthogonalize": ([C.POINTER(OrthoConfig), C.POINTER(C.c_float), C.c_void_p, C.c_int, C.c_long, C.c_void_p, C.c_int, C.c_long,
+                          C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
     "rl_gemm_f32": ([C.POINTER(_GemmConfigC), C.c_void_p, C.c_void_p, C.c_void_p] + [C.c_int] * 6 + [C.c_void_p], C.c_int),
 }
 
