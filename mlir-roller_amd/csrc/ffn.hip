@@ -123,8 +123,8 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
   return r;
 }
 
-template <int BLOCKS, int SPLIT>
-int few_rows(const FfnCall& c, const void* h, const GatedForward<T>& gated, const Store<T>& out, int pitch) {
+template <int BLOCKS, int SPLIT, int KIND>
+int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated, const Store<T>& out, int pitch) {
   // Enough waves to keep the memory busy from every CU: up to 16 share the K of 16 weight rows, none with
   // fewer than 256 bytes of each row.
   auto waves = [&](int groups, int K) {
@@ -134,7 +134,7 @@ int few_rows(const FfnCall& c, const void* h, const GatedForward<T>& gated, cons
   };
   typedef typename x_type<T, SPLIT>::type H;
   const int up = (pitch + 15) / 16, down = (c.D + 15) / 16;
-  PT_TRY(launch(few_rows_kernel<T, BLOCKS, 1, 0, GatedForward<T>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
+  PT_TRY(launch(few_rows_kernel<T, BLOCKS, 1, 0, GatedForward<T, KIND>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
                 (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, pitch, c.D, gated));
   return launch(few_rows_kernel<T, BLOCKS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
                 c.D, c.D, c.F, out);
@@ -142,18 +142,18 @@ int few_rows(const FfnCall& c, const void* h, const GatedForward<T>& gated, cons
 
 size_t forward_room(const FfnCall& c, bool unaligned) { return forward_carve(c, unaligned).bytes; }
 
-int forward(const FfnCall& call) {
+template <int KIND>
+int forward_as(const FfnCall& call) {
   FfnCall c = call;
   const ForwardRoom r = forward_carve(c, false);
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
   T* h = c.saved ? (T*)((char*)c.saved + s.h) : r.h;
-  GatedForward<T> gated = {};
+  GatedForward<T, KIND> gated = {};
   gated.h = h;
   gated.h32 = r.h32;
   gated.g = c.saved ? (float*)((char*)c.saved + s.g) : nullptr;
   gated.u = c.saved ? (float*)((char*)c.saved + s.u) : nullptr;
   gated.pitch = s.pitch;
-  gated.kind = c.activation;
   const Store<T> out = store(c.y, c.ldy, c.D);
   if (c.T <= 16) return few_rows<1, SPLIT_TOKENS != 0>(c, r.h32 ? (const void*)r.h32 : h, gated, out, s.pitch);
   if (c.T <= 32) return few_rows<2, 0>(c, h, gated, out, s.pitch);
@@ -169,6 +169,10 @@ int forward(const FfnCall& call) {
   PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: gate and up")));
   const Problem down = problem(h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
   return run_product<T, 1, 1, 0, 1, 0>(down, out, 1, r.slabs, c.stream, c.compute_units, "ffn: down");
+}
+
+int forward(const FfnCall& c) {
+  return c.activation == ACT_SILU ? forward_as<ACT_SILU>(c) : c.activation == ACT_GELU ? forward_as<ACT_GELU>(c) : forward_as<ACT_GELU_TANH>(c);
 }
 
 // ---- backward ----
@@ -209,6 +213,17 @@ int zero(void* p, int ld, int rows, int cols, hipStream_t stream) {
   return launch(zero_kernel<T>, "ffn: zero gradient", dim3(blocks_for((long)rows * cols)), 256, stream, (T*)p, ld, rows, cols);
 }
 
+template <int KIND>
+int gated_backward(const FfnCall& c, const BackwardRoom& r, const FfnSaved& s, const Problem& dh) {
+  GatedBackward<T, KIND> gated = {};
+  gated.g = (const float*)((char*)c.saved + s.g);
+  gated.u = (const float*)((char*)c.saved + s.u);
+  gated.dg = r.dg;
+  gated.du = r.du;
+  gated.pitch = s.pitch;
+  return run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: dh");
+}
+
 int backward(const FfnCall& call) {
   FfnCall c = call;
   if (c.T == 0) {   // no tokens: the gradients of the weights are zero
@@ -227,15 +242,12 @@ int backward(const FfnCall& call) {
   }
   if (!c.dx && !c.dw_gate) return RL_OK;
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
-  GatedBackward<T> gated = {};
-  gated.g = (const float*)((char*)c.saved + s.g);
-  gated.u = (const float*)((char*)c.saved + s.u);
-  gated.dg = r.dg;
-  gated.du = r.du;
-  gated.pitch = s.pitch;
-  gated.kind = c.activation;
   const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, s.pitch);
-  PT_TRY((run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: dh")));
+  switch (c.activation) {
+    case ACT_SILU: PT_TRY(gated_backward<ACT_SILU>(c, r, s, dh)); break;
+    case ACT_GELU: PT_TRY(gated_backward<ACT_GELU>(c, r, s, dh)); break;
+    default: PT_TRY(gated_backward<ACT_GELU_TANH>(c, r, s, dh)); break;
+  }
   if (c.dx) {
     PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
     PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));

@@ -1,7 +1,7 @@
 // Newton-Schulz orthogonalisation of a matrix or a stack of them:
 //   X0 = G / (||G||_F + eps);   A = X X^T, B = b A + c A^2, X <- a X + B X   (steps times);   O = scale X
 // with X the shorter side by the longer one (a tall G is worked on transposed).  A, A^2 and B are symmetric:
-// only the tiles on and below the diagonal are computed, and each writes its mirror image too.
+// only the tiles on and below the diagonal are computed, and those below it leave twice.
 //
 // Precision.  The iteration multiplies the small directions of X by a (3.4 by default) in every step, and
 // with them the rounding errors of what is multiplied: with bf16 operands the result is 1 to 20 % off, in
@@ -110,25 +110,20 @@ struct Symmetric {
   Op* off;        // [pitch][pitch]
   float* diag;    // [pitch]
   int pitch;
-  int tile;       // tile of the product: a tile off the diagonal writes its mirror image too
   __device__ __forceinline__ Symmetric of(int batch) const {
     Symmetric o = *this;
     o.off += (long)batch * pitch * pitch;
     o.diag += (long)batch * pitch;
     return o;
   }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const {
+  __device__ __forceinline__ void put(int m, int n, v4f v, bool ok) const {
     v4f x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (m == n + e) diag[m] = v[e];
+      if (ok && m == n + e) diag[m] = v[e];
       x[e] = m == n + e ? 0.0f : v[e] * kScale<Op>;
     }
-    store4(off + (long)m * pitch + n, x);
-    if (m / tile != n / tile) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) off[(long)(n + e) * pitch + m] = (Op)x[e];
-    }
+    if (ok) store4(off + (long)m * pitch + n, x);
   }
 };
 
@@ -137,7 +132,9 @@ template <class Op>
 struct Gram {
   Symmetric<Op> A;
   __device__ __forceinline__ Gram at(int batch, int) const { return {A.of(batch)}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const { A.put(m, n, v * (1.0f / (kScale<Op> * kScale<Op>))); }
+  struct In {};
+  __device__ __forceinline__ In get(int, int) const { return {}; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const { A.put(m, n, v * (1.0f / (kScale<Op> * kScale<Op>)), ok); }
 };
 
 // B = b A + c A^2, from the product of Ao with itself
@@ -146,17 +143,21 @@ struct Polynomial {
   Symmetric<Op> A, B;
   float b, c;
   __device__ __forceinline__ Polynomial at(int batch, int) const { return {A.of(batch), B.of(batch), b, c}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const {
-    const v4f ao = load4(A.off + (long)m * A.pitch + n) * (1.0f / kScale<Op>);
-    const v4f dn = *(const v4f*)(A.diag + n);
-    const float dm = A.diag[m];
+  struct In {
+    v4f ao, dn;
+    float dm;
+  };
+  __device__ __forceinline__ In get(int m, int n) const { return {load4(A.off + (long)m * A.pitch + n), *(const v4f*)(A.diag + n), A.diag[m]}; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In in, bool ok) const {
+    const v4f ao = in.ao * (1.0f / kScale<Op>), dn = in.dn;
+    const float dm = in.dm;
     v4f x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float sq = v[e] * (1.0f / (kScale<Op> * kScale<Op>));
       x[e] = m == n + e ? b * dm + c * (sq + dm * dm) : b * ao[e] + c * (sq + (dm + dn[e]) * ao[e]);
     }
-    B.put(m, n, x);
+    B.put(m, n, x, ok);
   }
 };
 
@@ -181,9 +182,15 @@ struct Update {
     o.diag += (long)batch * diag_pitch;
     return o;
   }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const {
+  struct In {
+    v4f x;
+    float d;
+  };
+  __device__ __forceinline__ In get(int m, int n) const { return {*(const v4f*)(from + (long)m * pitch + n), diag[m]}; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In in, bool ok) const {
     const long i = (long)m * pitch + n;
-    const v4f x = *(const v4f*)(from + i) * (a + diag[m]) + v * (1.0f / (kScale<Op> * kScale<Op>));
+    const v4f x = in.x * (a + in.d) + v * (1.0f / (kScale<Op> * kScale<Op>));
+    if (!ok) return;
     if (out) {
       T* o = out + (long)m * ldo + n;
       if (vec && n + 3 < l) {
@@ -274,14 +281,12 @@ int run(const OrthoCall& c) {
     p.M_out = p.N_out = r.sq;
     p.K = r.l;
     p.batch_a = p.batch_b = x_stride;
-    Symmetric<Op> A = {(Op*)r.ao, r.da, r.sq, 0}, B = {(Op*)r.bo, r.db, r.sq, 0};
-    A.tile = kTiles[plan_product(sizeof(Op), 0, 1, 1, r.sq, r.sq, r.l, c.batch, c.compute_units).tile].bm;
+    Symmetric<Op> A = {(Op*)r.ao, r.da, r.sq}, B = {(Op*)r.bo, r.db, r.sq};
     PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Gram<Op>{A}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: X X^T")));
     p.a[0] = p.b[0] = r.ao;
     p.lda = p.ldb = p.ldb1 = r.sq;
     p.K = r.s;
     p.batch_a = p.batch_b = (long)r.sq * r.sq;
-    B.tile = kTiles[plan_product(sizeof(Op), 0, 1, 1, r.sq, r.sq, r.s, c.batch, c.compute_units).tile].bm;
     PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Polynomial<Op>{A, B, b, cc}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: A A")));
     const int next = 1 - cur;
     Update<T, Op> u = {};

@@ -34,15 +34,16 @@ inline unsigned blocks_for(long items) {
 // Tile k of kTiles (product_plan.h): BM x BN, wave tile, workgroups per CU.
 template <int K>
 struct tile;
-template <> struct tile<0> { static constexpr int BM = 256, BN = 256, WM = 128, WN = 128, PER_CU = 1; };
-template <> struct tile<1> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 2; };
-template <> struct tile<2> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 4; };
+template <> struct tile<0> { static constexpr int BM = 256, BN = 256, WM = 128, WN = 128, PER_CU = 1, BUFS = 2; };
+template <> struct tile<1> { static constexpr int BM = 192, BN = 192, WM = 96, WN = 96, PER_CU = 1, BUFS = 3; };
+template <> struct tile<2> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 2, BUFS = 2; };
+template <> struct tile<3> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 4, BUFS = 2; };
 
 template <int K, class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
 int launch_tile(const Problem& p, const Partial& part, const Epi& epi, int batch, hipStream_t stream, const char* what) {
   typedef tile<K> t;
-  // a gated wave tile of 32 columns is 16 of each kind: blocks of 16
-  typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, (GATED && t::WN < 64) ? 16 : 32> S;
+  // a gated wave tile of 32 or 96 columns is 16 or 48 of each kind: blocks of 16
+  typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, (GATED && t::WN / 2 % 32 != 0) ? 16 : 32, t::BUFS> S;
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits;
   if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
@@ -64,7 +65,8 @@ int run_product(Problem p, const Epi& epi, int batch, void* room, hipStream_t st
   switch (plan.tile) {
     case 0: PT_TRY((launch_tile<0, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
     case 1: PT_TRY((launch_tile<1, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
-    default: PT_TRY((launch_tile<2, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
+    case 2: PT_TRY((launch_tile<2, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
+    default: PT_TRY((launch_tile<3, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
   }
   if (p.splits == 1) return RL_OK;
   const long quads = (long)p.M_out * (part.pitch / 4);

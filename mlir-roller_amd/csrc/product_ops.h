@@ -1,9 +1,9 @@
 // What follows a product: the epilogues of the matrix-product engine (product_tile.h) for the gated
 // feed-forward block and for Newton-Schulz orthogonalisation, and the small kernels around them.
 //
-// An epilogue is a struct with at(batch, split), which picks the buffers of a batch entry, and
-// put(m, n, v): four consecutive columns n .. n+3 of row m, n a multiple of 4 (gated products:
-// put(m, n, gate, up)).
+// An epilogue is a struct with at(batch, split), which picks the buffers of a batch entry, get(m, n), which
+// loads what it needs besides the product, and put(m, n, v, in, ok): four consecutive columns n .. n+3 of row
+// m, n a multiple of 4 (gated products: put(m, n, gate, up, in, ok)), stored if ok.
 
 #ifndef PRODUCT_OPS_H
 #define PRODUCT_OPS_H
@@ -46,21 +46,23 @@ PT_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_am
 
 constexpr float GELU_2C = 1.5957691216f, GELU_C1 = 0.044715f;   // 2 sqrt(2 / pi)
 
-PT_DEV float act(int kind, float g) {
-  if (kind == ACT_SILU) return g * sigmoid(g);
-  if (kind == ACT_GELU) return 0.5f * g * (1.0f + erff(0.70710678f * g));
+template <int KIND>
+PT_DEV float act(float g) {
+  if constexpr (KIND == ACT_SILU) return g * sigmoid(g);
+  if constexpr (KIND == ACT_GELU) return 0.5f * g * (1.0f + erff(0.70710678f * g));
   return g * sigmoid(GELU_2C * (g + GELU_C1 * g * g * g));   // (1 + tanh z) / 2 = sigmoid(2 z)
 }
 
 // The activation and its slope.  The factors that grow with g stand beside ones that have long been zero
 // where they would overflow, so they are taken of g cut to +-32.
-PT_DEV void act_slope(int kind, float g, float& a, float& slope) {
+template <int KIND>
+PT_DEV void act_slope(float g, float& a, float& slope) {
   const float c = fminf(fmaxf(g, -32.0f), 32.0f);
-  if (kind == ACT_SILU) {
+  if constexpr (KIND == ACT_SILU) {
     const float s = sigmoid(g);
     a = g * s;
     slope = s * (1.0f + c * (1.0f - s));
-  } else if (kind == ACT_GELU) {
+  } else if constexpr (KIND == ACT_GELU) {
     const float s = 0.5f * (1.0f + erff(0.70710678f * g));
     a = g * s;
     slope = s + c * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * c * c);
@@ -87,7 +89,10 @@ struct Store {
     }
     return o;
   }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const {
+  struct In {};
+  __device__ __forceinline__ In get(int, int) const { return {}; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const {
+    if (!ok) return;
     T* to = c[0] + (long)m * ldc + n;
     if (vec && n + 3 < N) {
       store4(to, v);
@@ -101,18 +106,21 @@ struct Store {
 
 // h = act(g) u; for a later backward pass g and u as well, unrounded (a gradient made of g and u rounded
 // to 16 bits would carry two or three roundings where it now carries its own).
-template <class T>
+template <class T, int KIND>
 struct GatedForward {
   T* h;           // NULL: only h32
   float* h32;     // h unrounded, NULL: not needed
   float *g, *u;   // NULL: not kept
-  int pitch, kind;
+  int pitch;
   __device__ __forceinline__ GatedForward at(int, int) const { return *this; }
-  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up) const {
+  struct In {};
+  __device__ __forceinline__ In get(int, int) const { return {}; }
+  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up, In, bool ok) const {
     const long i = (long)m * pitch + n;
     v4f o;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = act(kind, gate[e]) * up[e];
+    for (int e = 0; e < 4; ++e) o[e] = act<KIND>(gate[e]) * up[e];
+    if (!ok) return;
     if (h) store4(h + i, o);
     if (h32) *(v4f*)(h32 + i) = o;
     if (g) {
@@ -123,23 +131,30 @@ struct GatedForward {
 };
 
 // From dh: dg = dh u act'(g), du = dh act(g).
-template <class T>
+template <class T, int KIND>
 struct GatedBackward {
   const float *g, *u;
   T *dg, *du;
-  int pitch, kind;
+  int pitch;
   __device__ __forceinline__ GatedBackward at(int, int) const { return *this; }
-  __device__ __forceinline__ void put(int m, int n, v4f dh) const {
+  struct In {
+    v4f gate, up;
+  };
+  __device__ __forceinline__ In get(int m, int n) const {
     const long i = (long)m * pitch + n;
-    const v4f gate = *(const v4f*)(g + i), up = *(const v4f*)(u + i);
+    return {*(const v4f*)(g + i), *(const v4f*)(u + i)};
+  }
+  __device__ __forceinline__ void put(int m, int n, v4f dh, In in, bool ok) const {
+    const long i = (long)m * pitch + n;
     v4f x, y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float a, slope;
-      act_slope(kind, gate[e], a, slope);
-      x[e] = dh[e] * up[e] * slope;
+      act_slope<KIND>(in.gate[e], a, slope);
+      x[e] = dh[e] * in.up[e] * slope;
       y[e] = dh[e] * a;
     }
+    if (!ok) return;
     store4(dg + i, x);
     store4(du + i, y);
   }
@@ -147,24 +162,30 @@ struct GatedBackward {
 
 // ---- small kernels ----------------------------------------------------------------------------------
 
-// Sums the slabs of a split product in split order and hands them to the epilogue.
+// Sums the slabs of a split product in split order and hands them to the epilogue.  `tile`: the product is
+// symmetric and has no tiles of that size above its diagonal, where the mirror image is taken.
 template <class Epi, bool TWO>
 __global__ __launch_bounds__(256) void join_kernel(const Partial part, int splits, int tile, int M_out, int N_out, const Epi epi) {
   const int quads = (N_out + 3) / 4;
   const auto out = epi.at(blockIdx.z, 0);
   for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)M_out * quads; i += gridDim.x * 256L) {
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
-    if (tile && n / tile > m / tile) continue;   // (a symmetric product has no tiles above its diagonal)
-    const float* p = part.slab + (long)blockIdx.z * part.slab_size + (long)m * part.pitch + n;
-    v4f v = *(const v4f*)p, w = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (TWO) w = *(const v4f*)(p + part.slab_size);
-    for (int s = 1; s < splits; ++s) {
+    const float* p = part.slab + (long)blockIdx.z * part.slab_size;
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f}, w = v;
+    const bool above = tile && n / tile > m / tile;
+    for (int s = 0; s < splits; ++s) {
+      if (above) {
+        const float* q = p + (long)n * part.pitch + m;
+        v += v4f{q[0], q[part.pitch], q[2L * part.pitch], q[3L * part.pitch]};
+      } else {
+        const float* q = p + (long)m * part.pitch + n;
+        v += *(const v4f*)q;
+        if constexpr (TWO) w += *(const v4f*)(q + part.slab_size);
+      }
       p += part.per_split * part.slab_size;
-      v += *(const v4f*)p;
-      if constexpr (TWO) w += *(const v4f*)(p + part.slab_size);
     }
-    if constexpr (TWO) out.put(m, n, v, w);
-    else out.put(m, n, v);
+    if constexpr (TWO) out.put(m, n, v, w, out.get(m, n), true);
+    else out.put(m, n, v, out.get(m, n), true);
   }
 }
 
@@ -317,9 +338,9 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (n + e >= N) g[e] = u[e] = 0.0f;
-      out.put(m, n, g, u);
+      out.put(m, n, g, u, out.get(m, n), true);
     } else {
-      out.put(m, n, total[0][b]);
+      out.put(m, n, total[0][b], out.get(m, n), true);
     }
   }
 }

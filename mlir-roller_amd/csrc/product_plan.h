@@ -17,6 +17,7 @@ struct TileCost {
 
 constexpr TileCost kTiles[] = {
     {256, 256, 1, 0.80f, 1500.0f, 9000.0f},
+    {192, 192, 1, 0.75f, 1500.0f, 7000.0f},
     {128, 128, 2, 0.60f, 1200.0f, 5000.0f},
     {64, 64, 4, 0.35f, 1000.0f, 3500.0f},
 };
@@ -32,7 +33,7 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
   const int kstep = 128 / elem_bytes;
   const int steps = (K + kstep - 1) / kstep * segs;
   const float flops_per_cycle = elem_bytes == 2 ? 4096.0f : 256.0f;   // of one CU
-  for (int t = 0; t < 3; ++t) {
+  for (int t = 0; t < 4; ++t) {
     const TileCost& c = kTiles[t];
     const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + (gated ? c.bn / 2 : c.bn) - 1) / (gated ? c.bn / 2 : c.bn);
     const long tiles = (sym ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch;

@@ -26,9 +26,9 @@
 // block: a lane then holds four consecutive columns of one row of the result, and stores are
 // vectors.
 //
-// The K loop is software pipelined over two LDS buffers: the loads of step k+1 are in flight while
-// step k is multiplied, the fragments of the next 128-byte half are read beside the MFMAs of the
-// current one, also across the barrier between steps.
+// The K loop is software pipelined over two or three LDS buffers: the loads of the next steps are in
+// flight while a step is multiplied, and the fragments of the next MFMAs are read beside the current
+// ones, also across the barrier between steps.
 
 #ifndef PRODUCT_TILE_H
 #define PRODUCT_TILE_H
@@ -57,9 +57,23 @@ struct int_c {
   static constexpr int value = V;
 };
 
-PT_DEV __amdgpu_buffer_rsrc_t live_rsrc(const void* p, bool live) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, live ? 0x7fffffff : 0, 0x00020000);
+// Buffer resource over the 2 GiB from p, or over nothing: then a load returns 0 and touches no memory.
+PT_DEV v4u resource(const void* p, bool live) {
+  const unsigned long at = (unsigned long)p;
+  return v4u{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, live ? 0x7fffffffu : 0u, 0x00020000u};
 }
+
+#if __HIP_DEVICE_COMPILE__
+// 16 bytes per lane from `off` of the resource to LDS, lane by lane from `lds_at` on.  Written out, because
+// the compiler waits for a builtin load of this kind to land before it issues any ds_read_b64_tr_b16, to
+// whatever address; the K loop waits where a buffer changes hands.  (The instruction has no register
+// result; m0 needs one wait state before it.)
+PT_DEV void load_to_lds(v4u rsrc, unsigned lds_at, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_at), "v"(off), "s"(rsrc) : "m0");
+}
+// Waits until at most n of this wave's loads are outstanding (vmcnt is split over bits 3:0 and 15:14).
+#define wait_loads(n) __builtin_amdgcn_s_waitcnt(0x0f70 | ((n) & 0xf) | (((n) >> 4) << 14))
+#endif
 
 // One 16-byte fragment of each operand into an accumulator block of MI x MI.
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -74,15 +88,12 @@ template <class T, int MI>
 struct mma {
   static constexpr int PER_FRAG = sizeof(T) == 4 ? 4 : 1;
   typedef typename block<MI>::type acc_t;
-  PT_DEV acc_t run(v4u a, v4u b, acc_t c) {
+  // part t of PER_FRAG
+  PT_DEV acc_t part(int t, v4u a, v4u b, acc_t c) {
     if constexpr (sizeof(T) == 4) {
       const v4f x = __builtin_bit_cast(v4f, a), y = __builtin_bit_cast(v4f, b);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if constexpr (MI == 16) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], y[t], c, 0, 0, 0);
-        else c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[t], y[t], c, 0, 0, 0);
-      }
-      return c;
+      if constexpr (MI == 16) return __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], y[t], c, 0, 0, 0);
+      else return __builtin_amdgcn_mfma_f32_32x32x2f32(x[t], y[t], c, 0, 0, 0);
     } else if constexpr (__is_same(T, half_t)) {
       const v8h x = __builtin_bit_cast(v8h, a), y = __builtin_bit_cast(v8h, b);
       if constexpr (MI == 16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
@@ -92,6 +103,11 @@ struct mma {
       if constexpr (MI == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
       else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
     }
+  }
+  PT_DEV acc_t run(v4u a, v4u b, acc_t c) {
+#pragma unroll
+    for (int t = 0; t < PER_FRAG; ++t) c = part(t, a, b, c);
+    return c;
   }
 };
 
@@ -118,6 +134,11 @@ PT_DEV constexpr int mn_swizzle(int k) {
 template <class V>
 PT_DEV V lds_read(unsigned at) {
   return *(const __attribute__((address_space(3))) V*)at;
+}
+
+template <class V>
+PT_DEV void lds_write(unsigned at, V v) {
+  *(__attribute__((address_space(3))) V*)at = v;
 }
 
 // Address, within a row-major tile with rows of ROW_BYTES, of what a lane reads of the 32 rows from `row0`.
@@ -166,43 +187,31 @@ struct Problem {
 //   GATED       the tile's columns are BN/2 gate columns and the same BN/2 up columns, laid out so that
 //               a lane has both of a column (accumulator blocks j and j + TN/2)
 //   SEGS        K segments
-//   SYM         the result is symmetric: only the tiles on and below the diagonal exist
-template <class T_, int BM_, int BN_, int WM_, int WN_, int A_KM_, int B_KM_, int GATED_ = 0, int SEGS_ = 1, int SYM_ = 0, int PER_CU_ = 1, int MI_ = 32>
+//   SYM         the result is symmetric: only the tiles on and below the diagonal are computed, and those
+//               below it leave twice, as they are and transposed (M_out = N_out, a multiple of 4)
+template <class T_, int BM_, int BN_, int WM_, int WN_, int A_KM_, int B_KM_, int GATED_ = 0, int SEGS_ = 1, int SYM_ = 0, int PER_CU_ = 1, int MI_ = 32, int BUFS_ = 2>
 struct Shape {
   typedef T_ T;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, A_KM = A_KM_, B_KM = B_KM_, GATED = GATED_, SEGS = SEGS_, SYM = SYM_;
   static constexpr int PER_CU = PER_CU_;   // workgroups that should fit a CU
+  // Quarters of a step's loads that are issued a step ahead.  More wait out more latency, fewer crowd the
+  // end of a step less (8192^3 in bf16, K-major operands, 0 to 4: 1275, 1340, 1367, 1332, 1300 TFLOP/s).
+  static constexpr int TAIL_LOADS = 2;
   static constexpr int NWM = BM / WM, NWN = BN / WN, WAVES = NWM * NWN, NT = 64 * WAVES;
   static constexpr int ES = sizeof(T), KSTEP = STEP_BYTES / ES;
   static constexpr int MI = MI_, TM = WM / MI, TN = WN / MI;
   static constexpr int ROUNDS = MI / 8;               // fragment rounds per K step: each takes 64 / MI of its 8 chunks
   static constexpr int A_BYTES = BM * STEP_BYTES, B_BYTES = BN * STEP_BYTES;
-  static constexpr int LDS_BYTES = 2 * (A_BYTES + B_BYTES);
+  static constexpr int BUFS = BUFS_, LDS_BYTES = BUFS * (A_BYTES + B_BYTES);
   static constexpr int A_LOADS = BM * 8 / NT, B_LOADS = BN * 8 / NT;
   static constexpr int OUT_N = GATED ? BN / 2 : BN;   // result columns per tile
   static_assert(BM % WM == 0 && BN % WN == 0 && WM % MI == 0 && WN % MI == 0, "tile");
   static_assert((BM * 8) % NT == 0 && (BN * 8) % NT == 0, "whole loads per thread");
   static_assert(!GATED || ((WN / 2) % MI == 0 && B_KM), "gate and up halves of a wave tile");
   static_assert(!SYM || BM == BN, "square tiles");
+  static_assert(BUFS == 2 || BUFS == 3, "LDS buffers");
   static_assert(MI == 32 || (A_KM && B_KM), "row-major tiles are read 32 rows at a time");
 };
-
-// Orders the next NM MFMAs and NO instructions of class MASK evenly (0x100 LDS read, 0x020 global read).
-template <int NM, int NO, int MASK>
-PT_DEV void interleave() {
-  if constexpr (NM > 0) {
-    constexpr int q = NO / NM, rem = NO % NM;
-#pragma unroll
-    for (int i = 0; i < NM; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (i < rem) {
-        __builtin_amdgcn_sched_group_barrier(MASK, q + 1, 0);
-      } else if (q > 0) {
-        __builtin_amdgcn_sched_group_barrier(MASK, q > 0 ? q : 1, 0);
-      }
-    }
-  }
-}
 
 // Tile of a workgroup: every XCD gets a contiguous run of the tile order (workgroups are dealt to the
 // XCDs round-robin), and the order walks panels of 8 tile rows, so that neighbours share operand panels
@@ -223,13 +232,28 @@ PT_DEV void panel_tile(int pid, int nbm, int nbn, int& tm, int& tn) {
   tn = pid % width / rows;
 }
 
-// tile number p of the lower triangle, row by row: (p's row, column)
-PT_DEV void triangle_tile(int p, int& tm, int& tn) {
-  int r = (int)((__builtin_sqrtf(8.0f * (float)p + 1.0f) - 1.0f) * 0.5f);
-  while ((long)(r + 1) * (r + 2) / 2 <= p) ++r;
-  while ((long)r * (r + 1) / 2 > p) --r;
-  tm = r;
-  tn = p - (int)((long)r * (r + 1) / 2);
+// Tile number p of the lower triangle of n x n tiles, in panels of 8 tile rows: a panel's full columns one
+// after the other, 8 tiles each, then the triangle at its end, row by row.
+PT_DEV void triangle_tile(int p, int n, int& tm, int& tn) {
+  constexpr int GROUP = 8;
+  int g = 0, height = n < GROUP ? n : GROUP;
+  for (;;) {   // (a few panels)
+    const int size = GROUP * g * height + height * (height + 1) / 2;
+    if (p < size) break;
+    p -= size;
+    ++g;
+    height = n - GROUP * g < GROUP ? n - GROUP * g : GROUP;
+  }
+  if (p < GROUP * g * height) {
+    tm = GROUP * g + p % height;
+    tn = p / height;
+    return;
+  }
+  p -= GROUP * g * height;
+  int r = 0;
+  while (p > r) p -= ++r;
+  tm = GROUP * g + r;
+  tn = GROUP * g + p;
 }
 
 // Part of a split product: fp32, one slab of rows x pitch per split and batch entry (GATED: two, gate and up).
@@ -243,10 +267,14 @@ struct Partial {
     o.slab += ((long)split * per_split + batch) * slab_size;
     return o;
   }
-  __device__ __forceinline__ void put(int m, int n, v4f v) const { *(v4f*)(slab + (long)m * pitch + n) = v; }
-  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up) const {
-    put(m, n, gate);
-    *(v4f*)(slab + slab_size + (long)m * pitch + n) = up;
+  struct In {};
+  __device__ __forceinline__ In get(int, int) const { return {}; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const {
+    if (ok) *(v4f*)(slab + (long)m * pitch + n) = v;
+  }
+  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up, In in, bool ok) const {
+    put(m, n, gate, in, ok);
+    if (ok) *(v4f*)(slab + slab_size + (long)m * pitch + n) = up;
   }
 };
 
@@ -270,7 +298,7 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   pid = xcd_order(pid - split * tiles, tiles);
   int tile_m, tile_n;
   if constexpr (S::SYM) {
-    triangle_tile(pid, tile_m, tile_n);
+    triangle_tile(pid, nbm, tile_m, tile_n);
   } else {
     panel_tile(pid, nbm, nbn, tile_m, tile_n);
   }
@@ -286,12 +314,12 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
 
   // ---- what each lane fetches: offsets from the tile's first element, fixed through the K loop ----
   unsigned a_off[S::A_LOADS], b_off[S::B_LOADS];
-  int a_k, b_k[1];   // first k of the lane's chunks within a step (K-major: the same for every load of the lane)
+  int a_k;   // K-major: first k of the lane's chunks within a step, the same for every load
   // K-major: unit u is chunk (u % 8) ^ ((row / 2) % 8) of row u / 8; the rows of a lane's loads are NT / 8
   // apart, a multiple of 16, so the chunk is the same for all of them.
   static_assert(NT % 128 == 0 || (!S::A_KM && !S::B_KM), "the chunk of a lane's K-major loads is the same for all");
   const int km_chunk = (tid & 7) ^ ((tid >> 4) & 7);
-  a_k = b_k[0] = km_chunk * (16 / ES);
+  a_k = km_chunk * (16 / ES);
 #pragma unroll
   for (int i = 0; i < S::A_LOADS; ++i) {
     const int u = tid + i * NT;
@@ -329,10 +357,12 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   const long a_step = S::A_KM ? S::KSTEP : (long)S::KSTEP * p.lda;   // elements per K step
   const long b_step = S::B_KM ? S::KSTEP : (long)S::KSTEP * p.ldb;
 
-  // Issues the loads of K step kt (of this workgroup) into LDS buffer `buf`.  KTEST: the step may be one
-  // that K cuts short.  A step at or beyond KT gets an empty resource: zeros, no memory touched.
-  auto fetch = [&](auto ktest, int kt, int buf) __attribute__((always_inline)) {
-    constexpr bool KTEST = decltype(ktest)::value;
+  // Operand bases of K step kt (of this workgroup).  A step at or beyond KT gets empty resources.
+  struct source {
+    v4u a, b, b1;   // (b1: the up weights)
+    int k_left;     // of K, from the step's first k on
+  };
+  auto source_of = [&](int kt) __attribute__((always_inline)) {
     const bool live = kt < KT;
     int step = first_step + (live ? kt : 0), seg = 0;
     if constexpr (S::SEGS > 1) {
@@ -343,40 +373,29 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     }
     const T* ap = (const T*)(S::SEGS > 1 && seg == 1 ? p.a[1] : S::SEGS > 2 && seg == 2 ? p.a[2] : p.a[0]) + a_tile + step * a_step;
     const T* bp = (const T*)(S::SEGS > 1 && seg == 1 ? p.b[1] : S::SEGS > 2 && seg == 2 ? p.b[2] : p.b[0]) + b_tile + step * b_step;
-    const __amdgpu_buffer_rsrc_t ar = live_rsrc(ap, live), br = live_rsrc(bp, live);
-    const int k_left = p.K - step * S::KSTEP;
-    char* As = lds + buf * S::A_BYTES;
-    char* Bs = lds + 2 * S::A_BYTES + buf * S::B_BYTES;
-#pragma unroll
-    for (int i = 0; i < S::A_LOADS; ++i) {
+    source s;
+    s.a = resource(ap, live);
+    s.b = resource(bp, live);
+    if constexpr (S::GATED) s.b1 = resource((const T*)p.b[1] + b_tile1 + step * S::KSTEP, live);
+    s.k_left = p.K - step * S::KSTEP;
+    return s;
+  };
+  // Issues load i of a step (the loads of A, then those of B) into LDS buffer `buf`.  KTEST: the step may be
+  // one that K cuts short.
+  const unsigned lds0 = (unsigned)(unsigned long)(lds_ptr)lds;
+  auto load = [&](auto ktest, const source& s, int buf, int i) __attribute__((always_inline)) {
+    constexpr bool KTEST = decltype(ktest)::value;
+    if (i < S::A_LOADS) {
       unsigned off = a_off[i];
-      if constexpr (KTEST) {
-        if constexpr (S::A_KM) {
-          off = a_k < k_left ? off : OOB;
-        } else {
-          off = (tid + i * NT) / (S::BM * ES / 16) < k_left ? off : OOB;
-        }
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (lds_ptr)(As + (i * NT + wave * 64) * 16), 16, off, 0, 0, 0);
-    }
-    __amdgpu_buffer_rsrc_t br1 = br;
-    if constexpr (S::GATED) br1 = live_rsrc((const T*)p.b[1] + b_tile1 + step * S::KSTEP, live);
-#pragma unroll
-    for (int i = 0; i < S::B_LOADS; ++i) {
+      if constexpr (KTEST) off = (S::A_KM ? a_k : (tid + i * NT) / (S::BM * ES / 16)) < s.k_left ? off : OOB;
+      load_to_lds(s.a, lds0 + buf * S::A_BYTES + (i * NT + wave * 64) * 16, off);
+    } else {
+      i -= S::A_LOADS;
       unsigned off = b_off[i];
-      if constexpr (KTEST) {
-        if constexpr (S::B_KM) {
-          off = b_k[0] < k_left ? off : OOB;
-        } else {
-          off = (tid + i * NT) / (S::BN * ES / 16) < k_left ? off : OOB;
-        }
-      }
-      if constexpr (S::GATED) {
-        const int row = i * (NT / 8) + wave * 8;   // the 8 rows of this wave's load are all gate or all up
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(row % S::WN < S::WN / 2 ? br : br1, (lds_ptr)(Bs + (i * NT + wave * 64) * 16), 16, off, 0, 0, 0);
-      } else {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (lds_ptr)(Bs + (i * NT + wave * 64) * 16), 16, off, 0, 0, 0);
-      }
+      if constexpr (KTEST) off = (S::B_KM ? a_k : (tid + i * NT) / (S::BN * ES / 16)) < s.k_left ? off : OOB;
+      // (GATED: the 8 rows of a wave's load are all gate or all up)
+      const bool up = S::GATED && (i * (NT / 8) + wave * 8) % S::WN >= S::WN / 2;
+      load_to_lds(up ? s.b1 : s.b, lds0 + S::BUFS * S::A_BYTES + buf * S::B_BYTES + (i * NT + wave * 64) * 16, off);
     }
   };
 
@@ -405,32 +424,32 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   if constexpr (S::B_KM) {
 #pragma unroll
     for (int h = 0; h < ROUNDS; ++h) {
-      b_at[h] = 2 * S::A_BYTES + (wn0 + lr) * STEP_BYTES + ((64 / MI * h + lg) ^ ((lr >> 1) & 7)) * 16;
+      b_at[h] = S::BUFS * S::A_BYTES + (wn0 + lr) * STEP_BYTES + ((64 / MI * h + lg) ^ ((lr >> 1) & 7)) * 16;
       opaque(b_at[h]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      b_at[j] = 2 * S::A_BYTES + rows_at<ES, S::BN * ES>(wn0 + MI * j, lane);
+      b_at[j] = S::BUFS * S::A_BYTES + rows_at<ES, S::BN * ES>(wn0 + MI * j, lane);
       opaque(b_at[j]);
     }
   }
-  auto read = [&](frags& f, auto buf_c, auto round_c) __attribute__((always_inline)) {
+  // Fragment i of a round: blocks of A and B in the order in which the MFMAs ask for them.
+  auto read = [&](frags& f, auto buf_c, auto round_c, int i) __attribute__((always_inline)) {
     constexpr int buf = decltype(buf_c)::value, round = decltype(round_c)::value;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    if (i == 0 || i > TN) {
+      if (i) i -= TN;
       if constexpr (S::A_KM) {
         f.a[i] = lds_read<v4u>(a_at[round] + (buf * S::A_BYTES + i * MI * STEP_BYTES));
       } else {
         f.a[i] = read_rows<ES, S::BM * ES>(a_at[i] + (buf * S::A_BYTES + round * (S::KSTEP / ROUNDS) * S::BM * ES));
       }
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
+    } else {
+      i -= 1;
       if constexpr (S::B_KM) {
-        f.b[j] = lds_read<v4u>(b_at[round] + (buf * S::B_BYTES + j * MI * STEP_BYTES));
+        f.b[i] = lds_read<v4u>(b_at[round] + (buf * S::B_BYTES + i * MI * STEP_BYTES));
       } else {
-        f.b[j] = read_rows<ES, S::BN * ES>(b_at[j] + (buf * S::B_BYTES + round * (S::KSTEP / ROUNDS) * S::BN * ES));
+        f.b[i] = read_rows<ES, S::BN * ES>(b_at[i] + (buf * S::B_BYTES + round * (S::KSTEP / ROUNDS) * S::BN * ES));
       }
     }
   };
@@ -443,91 +462,171 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int r = 0; r < REGS; ++r) acc[i][j][r] = 0.0f;
-  auto multiply = [&](const frags& f, int i0, int i1) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = i0; i < i1; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mma<T, MI>::run(f.b[j], f.a[i], acc[i][j]);
-  };
 
   // ---- K loop ----
-  constexpr int G = TM * TN * mma<T, MI>::PER_FRAG;                // MFMAs per round
-  constexpr int RA = S::A_KM ? TM : TM * (ES == 2 ? 2 : 4), RB = S::B_KM ? TN : TN * (ES == 2 ? 2 : 4);
-  constexpr int R = RA + RB, L = S::A_LOADS + S::B_LOADS;
-  constexpr int EARLY = TM >= 4 ? TM / 4 : 0;                      // block rows multiplied before the barrier
+  // A step is ROUNDS rounds of G slots; a round multiplies one set of fragments while the next set is read.
+  // Buffer `cur` holds step kt, and the steps up to kt + BUFS - 1 are on their way into the others: of the
+  // last of them the first TAIL loads were issued at the end of step kt - 1, the others go out in the first
+  // two rounds.  A quarter into the last round the step's own reads are over and kt + 1 must have landed:
+  // the workgroup meets, reads the first fragments of kt + 1 and sends the first loads of kt + BUFS into
+  // `cur`.
+  // The order of instructions is the order written here (sched_barrier between the slots, one MFMA each, four with 32-bit operands):
+  // reads and loads are spread over the MFMAs, which run meanwhile; issued in a bunch they hold up the
+  // MFMAs behind them.
+  constexpr int PARTS = mma<T, MI>::PER_FRAG, G = TM * TN, FRAGS = TM + TN, L = S::A_LOADS + S::B_LOADS;
+  constexpr int BUFS = S::BUFS, EARLY = G / 4, TAIL = L * S::TAIL_LOADS / 4;
+  auto slot_mfma = [&](const frags& f, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = t * PARTS; e < (t + 1) * PARTS; ++e) {
+      const int i = e % G / TN, j = e % TN;
+      acc[i][j] = mma<T, MI>::part(e / G, f.b[j], f.a[i], acc[i][j]);
+    }
+  };
+  auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
   if (KT > 0) {
     frags f[2];
-    fetch(int_c<1>{}, 0, 0);
-    fetch(int_c<1>{}, 1, 1);
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (L & 0xf) | ((L >> 4) << 14));   // vmcnt <= L: step 0 has landed
+    {
+#pragma unroll
+      for (int b = 0; b < BUFS; ++b) {
+        const source s = source_of(b);
+#pragma unroll
+        for (int i = 0; i < (b + 1 < BUFS ? L : TAIL); ++i) load(int_c<1>{}, s, b, i);
+      }
+    }
+    wait_loads((BUFS - 2) * L + TAIL);   // step 0 has landed
     __syncthreads();
-    read(f[0], int_c<0>{}, int_c<0>{});
+#pragma unroll
+    for (int i = 0; i < FRAGS; ++i) read(f[0], int_c<0>{}, int_c<0>{}, i);
+    fence();
     auto step = [&](auto ktest, auto cur_c, int kt) __attribute__((always_inline)) {
       constexpr int cur = decltype(cur_c)::value;
-      read(f[1], cur_c, int_c<1>{});
-      multiply(f[0], 0, TM);
-      if constexpr (ROUNDS == 4) {
-        read(f[0], cur_c, int_c<2 % ROUNDS>{});
-        multiply(f[1], 0, TM);
-        read(f[1], cur_c, int_c<3 % ROUNDS>{});
-        multiply(f[0], 0, TM);
+      {
+        const source next = source_of(kt + BUFS - 1);
+        constexpr int into = (cur + BUFS - 1) % BUFS;
+        auto round = [&](auto round_c) __attribute__((always_inline)) {
+          constexpr int r = decltype(round_c)::value;
+          constexpr int FROM = TAIL + (r < 2 ? r : 2) * (L - TAIL) / 2, TO = TAIL + (r < 1 ? r + 1 : 2) * (L - TAIL) / 2;
+#pragma unroll
+          for (int t = 0; t < G; ++t) {
+            slot_mfma(f[r & 1], t);
+#pragma unroll
+            for (int i = t * FRAGS / G; i < (t + 1) * FRAGS / G; ++i) read(f[(r + 1) & 1], cur_c, int_c<r + 1>{}, i);
+#pragma unroll
+            for (int i = FROM + t * (TO - FROM) / G; i < FROM + (t + 1) * (TO - FROM) / G; ++i) load(ktest, next, into, i);
+            fence();
+          }
+        };
+        round(int_c<0>{});
+        if constexpr (ROUNDS == 4) {
+          round(int_c<ROUNDS - 3>{});
+          round(int_c<ROUNDS - 2>{});
+        } else {
+#pragma unroll
+          for (int i = TAIL + (L - TAIL) / 2; i < L; ++i) load(ktest, next, into, i);
+        }
       }
 #pragma unroll
-      for (int r = 1; r < ROUNDS; ++r) interleave<G, R, 0x100>();
-      multiply(f[1], 0, EARLY);
-      interleave<G * EARLY / TM, 0, 0x100>();
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt 0: step kt + 1 has landed
+      for (int t = 0; t < EARLY; ++t) slot_mfma(f[1], t);
+      fence();
+      wait_loads((BUFS - 2) * L);   // kt + 1 has landed
       __syncthreads();
-      read(f[0], int_c<1 - cur>{}, int_c<0>{});
-      fetch(ktest, kt + 2, cur);
-      multiply(f[1], EARLY, TM);
-      constexpr int REST = G - G * EARLY / TM;
-      interleave<(R < REST ? R : REST), R, 0x100>();
-      if constexpr (REST > R) interleave<REST - R, L, 0x020>();
-      __builtin_amdgcn_sched_barrier(0);
+      fence();
+      const source next = source_of(kt + BUFS);
+      constexpr int REST = G - EARLY;
+#pragma unroll
+      for (int t = 0; t < REST; ++t) {
+        slot_mfma(f[1], EARLY + t);
+#pragma unroll
+        for (int i = t * FRAGS / REST; i < (t + 1) * FRAGS / REST; ++i) read(f[0], int_c<(cur + 1) % BUFS>{}, int_c<0>{}, i);
+#pragma unroll
+        for (int i = t * TAIL / REST; i < (t + 1) * TAIL / REST; ++i) load(ktest, next, cur, i);
+        fence();
+      }
     };
     int kt = 0;
-    // steps whose fetch (of kt + 2) cannot be cut short by the end of K (of any segment)
-    const int cut_free = p.K % S::KSTEP == 0 ? KT : (S::SEGS > 1 ? 0 : (last_step == seg_steps ? KT - 3 : KT));
-    for (; kt + 1 < KT && kt + 1 < cut_free; kt += 2) {
-      step(int_c<0>{}, int_c<0>{}, kt);
-      step(int_c<0>{}, int_c<1>{}, kt + 1);
-    }
-    for (; kt + 1 < KT; kt += 2) {
-      step(int_c<1>{}, int_c<0>{}, kt);
-      step(int_c<1>{}, int_c<1>{}, kt + 1);
-    }
+    // steps none of whose loads (up to those of kt + BUFS) can be cut short by the end of K (of any segment)
+    const int cut_free = p.K % S::KSTEP == 0 ? KT : (S::SEGS > 1 ? 0 : (last_step == seg_steps ? KT - 1 - BUFS : KT));
+    auto pass = [&](auto ktest) __attribute__((always_inline)) {
+      step(ktest, int_c<0>{}, kt);
+      step(ktest, int_c<1>{}, kt + 1);
+      if constexpr (BUFS == 3) step(ktest, int_c<2>{}, kt + 2);
+      kt += BUFS;
+    };
+    while (kt + BUFS <= KT && kt + BUFS <= cut_free) pass(int_c<0>{});
+    while (kt + BUFS <= KT) pass(int_c<1>{});
     if (kt < KT) step(int_c<1>{}, int_c<0>{}, kt);
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // the empty requests past the end have drained
+    if constexpr (BUFS == 3) {
+      if (kt + 1 < KT) step(int_c<1>{}, int_c<1>{}, kt + 1);
+    }
+    wait_loads(0);   // the empty requests past the end have drained
   }
 
-  // ---- every accumulator leaves once: row m, columns n to n + 3 ----
-  auto leave = [&](auto out) __attribute__((always_inline)) {
+  // ---- every accumulator leaves once ----
+  // Through LDS, which the K loop has left: each wave writes a row of its blocks there (its own part, so
+  // no wave waits for another) and reads it back row by row, four columns a lane.  Stores and the
+  // epilogue's own loads are then whole stretches of a row, and its code is a loop instead of a copy per
+  // accumulator.  Rows are padded by 16 bytes: the 16-byte writes of the lanes of a block go to
+  // consecutive rows.
+  __syncthreads();
+  constexpr int PITCH = S::WN + 4;
+  static_assert(S::WAVES * MI * PITCH * 4 <= S::LDS_BYTES, "a row of blocks per wave fits the LDS");
+  const unsigned mine = wave * (MI * PITCH * 4);
+  const unsigned to = mine + (lr * PITCH + 4 * lg) * 4;
+  auto leave = [&](auto out, auto mirror) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int m = m0 + wm0 + i * MI + lr;
 #pragma unroll
-      for (int j = 0; j < (S::GATED ? TN / 2 : TN); ++j)
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int q = 0; q < REGS / 4; ++q) {
-          // registers 4q .. 4q+3 of lane group lg: columns 256 / MI * q + 4 * lg and on of the block
-          const int col = j * MI + 256 / MI * q + 4 * lg;
-          auto four = [&](int jj) __attribute__((always_inline)) { return v4f{acc[i][jj][4 * q], acc[i][jj][4 * q + 1], acc[i][jj][4 * q + 2], acc[i][jj][4 * q + 3]}; };
-          if constexpr (S::GATED) {
-            const int n = n0 + (wave % S::NWN) * (S::WN / 2) + col;
-            if (m < p.M_out && n < p.N_out) out.put(m, n, four(j), four(j + TN / 2));
-          } else {
-            const int n = n0 + wn0 + col;
-            if (m < p.M_out && n < p.N_out) out.put(m, n, four(j));
+        for (int q = 0; q < REGS / 4; ++q)   // registers 4q .. 4q+3: columns 256 / MI * q + 4 * lg and on of the block
+          lds_write(to + (j * MI + 256 / MI * q) * 4, v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+      const int mb = m0 + wm0 + i * MI;
+      constexpr int COLS = S::GATED ? S::WN / 2 : S::WN, PER_ROW = COLS / 4, UNITS = MI * PER_ROW;   // 4 columns a unit
+      const int nb = n0 + (S::GATED ? (wave % S::NWN) * (S::WN / 2) : wn0);
+      typedef typename decltype(out)::In In;
+      constexpr int PER_LANE = UNITS / 64, MOST = sizeof(In) > 32 ? 4 : 8;
+      constexpr int BATCH = PER_LANE <= MOST ? PER_LANE : PER_LANE % MOST == 0 ? MOST : PER_LANE % 6 == 0 ? 6 : 4;
+      static_assert(UNITS % 64 == 0 && PER_LANE % BATCH == 0, "whole batches");
+      // The epilogue's loads for BATCH units first (of the nearest unit that exists), then their results:
+      // the loads wait for memory together, and nothing but the stores is conditional.
+      auto units = [&](auto transposed) __attribute__((always_inline)) {
+        constexpr bool TR = decltype(transposed)::value;
+        constexpr int PER = TR ? MI / 4 : PER_ROW;
+        const int m_last = p.M_out - 1, n_last = (p.N_out - 1) / 4 * 4;
+#pragma unroll 1
+        for (int u0 = lane; u0 < UNITS; u0 += 64 * BATCH) {
+          In in[BATCH];
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            const int u = u0 + 64 * k, m = (TR ? nb : mb) + u / PER, n = (TR ? mb : nb) + u % PER * 4;
+            in[k] = out.get(m < m_last ? m : m_last, n < n_last ? n : n_last);
+          }
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            const int u = u0 + 64 * k, r = u / PER, c = u % PER * 4, m = (TR ? nb : mb) + r, n = (TR ? mb : nb) + c;
+            const bool ok = m <= m_last && n <= n_last;
+            const unsigned from = mine + (TR ? c * PITCH + r : r * PITCH + c) * 4;
+            if constexpr (S::GATED) {
+              out.put(m, n, lds_read<v4f>(from), lds_read<v4f>(from + S::WN / 2 * 4), in[k], ok);
+            } else if constexpr (TR) {
+              out.put(m, n, v4f{lds_read<float>(from), lds_read<float>(from + PITCH * 4), lds_read<float>(from + PITCH * 8), lds_read<float>(from + PITCH * 12)}, in[k], ok);
+            } else {
+              out.put(m, n, lds_read<v4f>(from), in[k], ok);
+            }
           }
         }
+      };
+      units(int_c<0>{});
+      // the mirror image of a tile below the diagonal: four rows of one column a unit
+      if constexpr (S::SYM && decltype(mirror)::value) {
+        if (tile_m != tile_n) units(int_c<1>{});
+      }
     }
   };
   if (p.splits > 1) {
-    leave(partial.at(batch, split));
+    leave(partial.at(batch, split), int_c<0>{});
   } else {
-    leave(epi.at(batch, 0));
+    leave(epi.at(batch, 0), int_c<1>{});
   }
 #endif
 }
