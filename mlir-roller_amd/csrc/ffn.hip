@@ -34,7 +34,7 @@ constexpr int ES = sizeof(T), PER = 16 / ES;
 constexpr int FEW = 64;   // tokens up to which the forward products take the few_rows kernel
 constexpr int SPLIT_TOKENS = ES == 2 ? 16 : 0;   // tokens up to which h goes into the second product unrounded
 
-int pitch_of(int n) { return (n + PER - 1) / PER * PER; }
+int pitch_of(int n) { return line_pitch(ES, n); }
 
 // The tile engine reads whole 16-byte chunks: a matrix whose rows are anything else is packed first.
 bool aligned(const FfnMatrix& m, int cols) { return (uintptr_t)m.p % 16 == 0 && m.ld % PER == 0 && cols % PER == 0; }
@@ -115,7 +115,7 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
     r.w_gate = pack_space(room, c.w_gate, c.F, c.D, unaligned || !aligned(c.w_gate, c.D));
     r.w_up = pack_space(room, c.w_up, c.F, c.D, unaligned || !aligned(c.w_up, c.D));
     r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
-    const size_t up = plan_product(ES, 1, 1, 0, c.T, s.pitch, c.D, 1, c.compute_units).slab_bytes;
+    const size_t up = plan_product(ES, 1, 1, 0, c.T, s.cols, c.D, 1, c.compute_units).slab_bytes;
     const size_t down = plan_product(ES, 0, 1, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes;
     r.slabs = room.take(larger(up, down));
   }
@@ -124,7 +124,7 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
 }
 
 template <int BLOCKS, int SPLIT, int KIND>
-int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated, const Store<T>& out, int pitch) {
+int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated, const Store<T>& out, const FfnSaved& s) {
   // Enough waves to keep the memory busy from every CU: up to 16 share the K of 16 weight rows, none with
   // fewer than 256 bytes of each row.
   auto waves = [&](int groups, int K) {
@@ -133,10 +133,10 @@ int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated
     return 64 * w;
   };
   typedef typename x_type<T, SPLIT>::type H;
-  const int up = (pitch + 15) / 16, down = (c.D + 15) / 16;
+  const int up = (s.cols + 15) / 16, down = (c.D + 15) / 16;
   PT_TRY(launch(few_rows_kernel<T, BLOCKS, 1, 0, GatedForward<T, KIND>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
-                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, pitch, c.D, gated));
-  return launch(few_rows_kernel<T, BLOCKS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
+                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, s.cols, c.D, gated));
+  return launch(few_rows_kernel<T, BLOCKS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
                 c.D, c.D, c.F, out);
 }
 
@@ -155,15 +155,15 @@ int forward_as(const FfnCall& call) {
   gated.u = c.saved ? (float*)((char*)c.saved + s.u) : nullptr;
   gated.pitch = s.pitch;
   const Store<T> out = store(c.y, c.ldy, c.D);
-  if (c.T <= 16) return few_rows<1, SPLIT_TOKENS != 0>(c, r.h32 ? (const void*)r.h32 : h, gated, out, s.pitch);
-  if (c.T <= 32) return few_rows<2, 0>(c, h, gated, out, s.pitch);
-  if (c.T <= FEW) return few_rows<4, 0>(c, h, gated, out, s.pitch);
+  if (c.T <= 16) return few_rows<1, SPLIT_TOKENS != 0>(c, r.h32 ? (const void*)r.h32 : h, gated, out, s);
+  if (c.T <= 32) return few_rows<2, 0>(c, h, gated, out, s);
+  if (c.T <= FEW) return few_rows<4, 0>(c, h, gated, out, s);
 
   PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
   PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
   PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
-  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, s.pitch);
+  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, s.cols);
   up.b[1] = c.w_up.p;
   up.ldb1 = c.w_up.ld;
   PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: gate and up")));
@@ -198,7 +198,7 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
   r.w_gate = pack_space(room, c.w_gate, c.F, c.D, weights);
   r.w_up = pack_space(room, c.w_up, c.F, c.D, weights);
   r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
-  size_t slabs = plan_product(ES, 0, 1, 0, c.T, s.pitch, c.D, 1, c.compute_units).slab_bytes;
+  size_t slabs = plan_product(ES, 0, 1, 0, c.T, s.cols, c.D, 1, c.compute_units).slab_bytes;
   slabs = larger(slabs, plan_product(ES, 0, 2, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes);
   slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.F, c.D, c.T, 2, c.compute_units).slab_bytes);
   slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.D, c.F, c.T, 1, c.compute_units).slab_bytes);
@@ -242,7 +242,7 @@ int backward(const FfnCall& call) {
   }
   if (!c.dx && !c.dw_gate) return RL_OK;
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
-  const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, s.pitch);
+  const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, s.cols);
   switch (c.activation) {
     case ACT_SILU: PT_TRY(gated_backward<ACT_SILU>(c, r, s, dh)); break;
     case ACT_GELU: PT_TRY(gated_backward<ACT_GELU>(c, r, s, dh)); break;

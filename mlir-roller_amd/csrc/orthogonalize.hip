@@ -48,9 +48,9 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, int ld, long stri
 }
 
 // X0 in fp32 and as an operand, 64 x 64 elements per workgroup, transposed if G is tall; zeros behind the
-// rows' ends up to the pitch.
+// rows' ends up to whole chunks.
 template <class T, class Op>
-__global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long stride, int tall, const double* partial, int n_partial, float eps, int s, int l, int pitch, long x_stride, float* X, Op* Xop) {
+__global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long stride, int tall, const double* partial, int n_partial, float eps, int s, int l, int l8, int pitch, long x_stride, float* X, Op* Xop) {
   __shared__ double total[256];
   __shared__ float patch[64][65];
   const int t = threadIdx.x;
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long str
   }
   for (int i = t / 64; i < 64; i += 4) {
     const int r = r0 + i, c = c0 + t % 64;
-    if (r >= s || c >= pitch) continue;
+    if (r >= s || c >= l8) continue;
     float v = tall ? patch[i][t % 64] : c < l ? (float)g[(long)r * ld + c] : 0.0f;
     v = v / norm;
     const long at = blockIdx.z * x_stride + (long)r * pitch + c;
@@ -107,12 +107,12 @@ __global__ __launch_bounds__(256) void out_kernel(const float* X, int s, int l, 
 // writes and the next ones read.
 template <class Op>
 struct Symmetric {
-  Op* off;        // [pitch][pitch]
+  Op* off;        // [rows][pitch]
   float* diag;    // [pitch]
-  int pitch;
+  int rows, pitch;
   __device__ __forceinline__ Symmetric of(int batch) const {
     Symmetric o = *this;
-    o.off += (long)batch * pitch * pitch;
+    o.off += (long)batch * rows * pitch;
     o.diag += (long)batch * pitch;
     return o;
   }
@@ -216,7 +216,9 @@ struct Room {
   float *da, *db;
   double* partial;
   char* slabs;
-  int s, l, pitch, sq;
+  int s, l;        // sides of X
+  int l8, s8;      // the same up to whole chunks: columns written
+  int pitch, sq;   // elements from row to row of X, and of A and B
   size_t bytes;
 };
 
@@ -234,9 +236,11 @@ Room carve(const OrthoCall& c) {
   };
   r.s = c.rows < c.cols ? c.rows : c.cols;
   r.l = c.rows < c.cols ? c.cols : c.rows;
-  r.pitch = (r.l + 7) / 8 * 8;
-  r.sq = (r.s + 7) / 8 * 8;
-  const size_t x = (size_t)c.batch * r.s * r.pitch, q = (size_t)c.batch * r.sq * r.sq;
+  r.l8 = (r.l + 7) / 8 * 8;
+  r.s8 = (r.s + 7) / 8 * 8;
+  r.pitch = line_pitch(sizeof(Op), r.l);
+  r.sq = line_pitch(sizeof(Op), r.s);
+  const size_t x = (size_t)c.batch * r.s * r.pitch, q = (size_t)c.batch * r.s8 * r.sq;
   r.x[0] = (float*)take(x * 4);
   if (sizeof(Op) == 2) {
     r.op[0] = (half_t*)take(x * 2);
@@ -249,9 +253,9 @@ Room carve(const OrthoCall& c) {
   r.da = (float*)take((size_t)c.batch * r.sq * 4);
   r.db = (float*)take((size_t)c.batch * r.sq * 4);
   r.partial = (double*)take((size_t)c.batch * NORM_BLOCKS * 8);
-  const size_t gram = plan_product(sizeof(Op), 0, 1, 1, r.sq, r.sq, r.l, c.batch, c.compute_units).slab_bytes;
-  const size_t poly = plan_product(sizeof(Op), 0, 1, 1, r.sq, r.sq, r.s, c.batch, c.compute_units).slab_bytes;
-  const size_t update = plan_product(sizeof(Op), 0, 1, 0, r.s, r.pitch, r.s, c.batch, c.compute_units).slab_bytes;
+  const size_t gram = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.l, c.batch, c.compute_units).slab_bytes;
+  const size_t poly = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.s, c.batch, c.compute_units).slab_bytes;
+  const size_t update = plan_product(sizeof(Op), 0, 1, 0, r.s, r.l8, r.s, c.batch, c.compute_units).slab_bytes;
   size_t slabs = gram > poly ? gram : poly;
   slabs = slabs > update ? slabs : update;
   r.slabs = take(slabs);
@@ -266,8 +270,8 @@ int run(const OrthoCall& c) {
   const long x_stride = (long)r.s * r.pitch;
   const int blocks = c.rows < 4 * NORM_BLOCKS ? (c.rows + 3) / 4 : NORM_BLOCKS;
   PT_TRY(launch(norm_kernel<T>, "orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial));
-  PT_TRY(launch(first_kernel<T, Op>, "orthogonalize: first X", dim3((r.pitch + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
-                r.s, r.l, r.pitch, x_stride, r.x[0], (Op*)r.op[0]));
+  PT_TRY(launch(first_kernel<T, Op>, "orthogonalize: first X", dim3((r.l8 + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
+                r.s, r.l, r.l8, r.pitch, x_stride, r.x[0], (Op*)r.op[0]));
   const int vec = (uintptr_t)c.o % (4 * sizeof(T)) == 0 && c.ldo % 4 == 0 && c.stride_o % 4 == 0;
   int cur = 0;
   for (int k = 0; k < c.steps; ++k) {
@@ -278,15 +282,15 @@ int run(const OrthoCall& c) {
     p.a[0] = p.b[0] = x;
     p.lda = p.ldb = p.ldb1 = r.pitch;
     p.M = p.N = r.s;
-    p.M_out = p.N_out = r.sq;
+    p.M_out = p.N_out = r.s8;
     p.K = r.l;
     p.batch_a = p.batch_b = x_stride;
-    Symmetric<Op> A = {(Op*)r.ao, r.da, r.sq}, B = {(Op*)r.bo, r.db, r.sq};
+    Symmetric<Op> A = {(Op*)r.ao, r.da, r.s8, r.sq}, B = {(Op*)r.bo, r.db, r.s8, r.sq};
     PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Gram<Op>{A}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: X X^T")));
     p.a[0] = p.b[0] = r.ao;
     p.lda = p.ldb = p.ldb1 = r.sq;
     p.K = r.s;
-    p.batch_a = p.batch_b = (long)r.sq * r.sq;
+    p.batch_a = p.batch_b = (long)r.s8 * r.sq;
     PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Polynomial<Op>{A, B, b, cc}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: A A")));
     const int next = 1 - cur;
     Update<T, Op> u = {};
@@ -309,7 +313,7 @@ int run(const OrthoCall& c) {
     p.ldb = p.ldb1 = r.pitch;
     p.N = r.l;
     p.M_out = r.s;
-    p.N_out = r.pitch;
+    p.N_out = r.l8;
     p.batch_b = x_stride;
     PT_TRY((run_product<Op, 1, 0, 0, 1, 0>(p, u, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: B X")));
     cur = next;

@@ -36,8 +36,8 @@ template <int K>
 struct tile;
 template <> struct tile<0> { static constexpr int BM = 256, BN = 256, WM = 128, WN = 128, PER_CU = 1, BUFS = 2; };
 template <> struct tile<1> { static constexpr int BM = 192, BN = 192, WM = 96, WN = 96, PER_CU = 1, BUFS = 3; };
-template <> struct tile<2> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 2, BUFS = 2; };
-template <> struct tile<3> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 4, BUFS = 2; };
+template <> struct tile<2> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 1, BUFS = 4; };
+template <> struct tile<3> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 2, BUFS = 4; };
 
 template <int K, class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
 int launch_tile(const Problem& p, const Partial& part, const Epi& epi, int batch, hipStream_t stream, const char* what) {

@@ -7,20 +7,29 @@
 
 namespace product {
 
+// What a tile costs on one compute unit, in microseconds: `step` per K step of 128 bytes, `fixed` for first
+// loads and epilogue, `once` for the launch.  Fitted to 840 timed products (64 to 5800 rows, 64 to 11000
+// columns, K 64 to 12000; K-major and row-major operands; 1 to 8 splits): the model is off by 4 to 13 % rms,
+// and what it chooses is on average 0.2 % slower, at worst 6 %, than the fastest choice timed.
+// The large tiles have the higher rate where they fill the CUs (4096^3 in bf16: 103 us with 256 x 256 tiles,
+// 113 with 192, 120 with 128, 191 with 64); the small ones where the others would not (1024 x 1920 x 5000:
+// 118, 65, 49 and 46 us unsplit), and 192 x 192 makes the lower triangle of 4096 x 4096 253 tiles for 256 CUs.
 struct TileCost {
-  int bm, bn;       // tile of the product (gated: bn / 2 result columns)
-  int per_cu;       // workgroups that share a CU
-  float rate;       // share of the matrix rate that a full CU reaches in the K loop
-  float step_floor; // cycles one K step takes at least: the round trip of its loads
-  float fixed;      // cycles per workgroup outside the K loop (first loads, epilogue)
+  int bm, bn;   // tile of the product (gated: bn / 2 result columns)
+  float step16, fixed16, once16;   // 16-bit operands
+  float step32, fixed32, once32;   // 32-bit operands
 };
 
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 0.80f, 1500.0f, 9000.0f},
-    {192, 192, 1, 0.75f, 1500.0f, 7000.0f},
-    {128, 128, 2, 0.60f, 1200.0f, 5000.0f},
-    {64, 64, 4, 0.35f, 1000.0f, 3500.0f},
+    {256, 256, 0.967f, 9.5f, 0.0f, 6.886f, 10.0f, 0.0f},
+    {192, 192, 0.554f, 7.6f, 0.0f, 3.872f, 7.8f, 0.0f},
+    {128, 128, 0.316f, 4.6f, 0.3f, 1.740f, 4.9f, 0.0f},
+    {64, 64, 0.159f, 1.0f, 2.8f, 0.448f, 1.2f, 2.4f},
 };
+constexpr float kJoinFixed = 4.5f;          // the launch that adds up a split product, microseconds
+constexpr float kSlabBytes = 3.5e6f;        // bytes of slabs written or read per microsecond
+constexpr int kMaxSplits = 16;
+constexpr size_t kMaxSlabs = (size_t)1 << 29;
 
 struct Plan {
   int tile, splits, steps_per_split;
@@ -32,29 +41,21 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
   float best_time = 0.0f;
   const int kstep = 128 / elem_bytes;
   const int steps = (K + kstep - 1) / kstep * segs;
-  const float flops_per_cycle = elem_bytes == 2 ? 4096.0f : 256.0f;   // of one CU
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < (int)(sizeof kTiles / sizeof kTiles[0]); ++t) {
     const TileCost& c = kTiles[t];
-    const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + (gated ? c.bn / 2 : c.bn) - 1) / (gated ? c.bn / 2 : c.bn);
+    const int out_n = gated ? c.bn / 2 : c.bn;
+    const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + out_n - 1) / out_n;
     const long tiles = (sym ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch;
-    const float step = 2.0f * c.bm * c.bn * kstep / flops_per_cycle / c.rate;   // alone on a CU at full rate
-    for (int splits = 1; splits <= 32; splits *= 2) {
+    const float step = elem_bytes == 2 ? c.step16 : c.step32, fixed = elem_bytes == 2 ? c.fixed16 : c.fixed32, once = elem_bytes == 2 ? c.once16 : c.once32;
+    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
       const int per = (steps + splits - 1) / splits;
-      if (splits > 1 && (per < 4 || (long)(splits - 1) * per >= steps)) break;
-      const long groups = tiles * splits;
-      const long slots = (long)compute_units * c.per_cu;
-      const long full = groups / slots, rest = groups % slots;
-      const float slots_f = (float)c.per_cu;
-      auto round = [&](float resident) {   // workgroups resident per CU
-        const float s = step * resident > c.step_floor ? step * resident : c.step_floor;
-        return per * s + c.fixed;
-      };
-      float time = full * round(slots_f);
-      if (rest) time += round((float)((rest + compute_units - 1) / compute_units));
+      // (every split has a step of its own, and two at least are worth a launch)
+      if (splits > 1 && (per < 2 || (long)(splits - 1) * per >= steps)) break;
       const size_t slab = splits > 1 ? (size_t)splits * batch * (gated ? 2 : 1) * M_out * ((N_out + 3) / 4 * 4) * 4 : 0;
-      // slabs: written once, read once, about 1.7 KB a cycle, and one more launch
-      if (splits > 1) time += 2.0f * slab / 1700.0f + 6000.0f;
-      if (slab > ((size_t)1 << 30)) break;
+      if (slab > kMaxSlabs) break;
+      const long per_cu = (tiles * splits + compute_units - 1) / compute_units;
+      float time = once + per_cu * (per * step + fixed);
+      if (splits > 1) time += kJoinFixed + 2.0f * slab / kSlabBytes;
       if (best_time == 0.0f || time < best_time) {
         best_time = time;
         best.tile = t;
@@ -65,6 +66,14 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
     }
   }
   return best;
+}
+
+// Pitch, in elements, of an internal matrix with rows of `cols`: an odd number of 128-byte lines.  Rows that
+// start inside a line cost an extra line per 128 bytes read (measured: 15 instead of 30 TB/s out of the L2),
+// and rows a power of two apart crowd the same memory channels (4.4 instead of 6.2 TB/s out of memory).
+inline int line_pitch(int elem_bytes, int cols) {
+  const int per_line = 128 / elem_bytes, lines = (cols + per_line - 1) / per_line;
+  return (lines | 1) * per_line;
 }
 
 }  // namespace product

@@ -26,7 +26,7 @@
 // block: a lane then holds four consecutive columns of one row of the result, and stores are
 // vectors.
 //
-// The K loop is software pipelined over two or three LDS buffers: the loads of the next steps are in
+// The K loop is software pipelined over two to four LDS buffers: the loads of the next steps are in
 // flight while a step is multiplied, and the fragments of the next MFMAs are read beside the current
 // ones, also across the barrier between steps.
 
@@ -209,7 +209,7 @@ struct Shape {
   static_assert((BM * 8) % NT == 0 && (BN * 8) % NT == 0, "whole loads per thread");
   static_assert(!GATED || ((WN / 2) % MI == 0 && B_KM), "gate and up halves of a wave tile");
   static_assert(!SYM || BM == BN, "square tiles");
-  static_assert(BUFS == 2 || BUFS == 3, "LDS buffers");
+  static_assert(BUFS >= 2 && BUFS <= 4, "LDS buffers");
   static_assert(MI == 32 || (A_KM && B_KM), "row-major tiles are read 32 rows at a time");
 };
 
@@ -549,14 +549,18 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     auto pass = [&](auto ktest) __attribute__((always_inline)) {
       step(ktest, int_c<0>{}, kt);
       step(ktest, int_c<1>{}, kt + 1);
-      if constexpr (BUFS == 3) step(ktest, int_c<2>{}, kt + 2);
+      if constexpr (BUFS > 2) step(ktest, int_c<2 % BUFS>{}, kt + 2);
+      if constexpr (BUFS > 3) step(ktest, int_c<3 % BUFS>{}, kt + 3);
       kt += BUFS;
     };
     while (kt + BUFS <= KT && kt + BUFS <= cut_free) pass(int_c<0>{});
     while (kt + BUFS <= KT) pass(int_c<1>{});
     if (kt < KT) step(int_c<1>{}, int_c<0>{}, kt);
-    if constexpr (BUFS == 3) {
+    if constexpr (BUFS > 2) {
       if (kt + 1 < KT) step(int_c<1>{}, int_c<1>{}, kt + 1);
+    }
+    if constexpr (BUFS > 3) {
+      if (kt + 2 < KT) step(int_c<1>{}, int_c<2>{}, kt + 2);
     }
     wait_loads(0);   // the empty requests past the end have drained
   }

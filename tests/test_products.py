@@ -60,10 +60,11 @@ def test_bf16_rounding():
 
 
 def test_saved_bytes(hip_lib):
-    # h in the element type, g and u in 32 bits, rows padded to 16 bytes, each part to 256 bytes
-    assert GatedFfn(64, 512, "bf16").saved_bytes(8) == 8 * 512 * (2 + 4 + 4)
-    assert GatedFfn(64, 510, "fp16").saved_bytes(8) == 8 * 512 * 10
-    assert GatedFfn(64, 510, "fp32").saved_bytes(2) == 3 * 2 * 512 * 4
+    # h in the element type, g and u in 32 bits; rows of an odd number of 128-byte lines of the element type,
+    # each part a multiple of 256 bytes
+    assert GatedFfn(64, 512, "bf16").saved_bytes(8) == 8 * 576 * (2 + 4 + 4)
+    assert GatedFfn(64, 510, "fp16").saved_bytes(8) == 8 * 576 * 10
+    assert GatedFfn(64, 510, "fp32").saved_bytes(2) == 3 * 4352        # 2 rows of 17 lines, 4352 bytes
     assert GatedFfn(64, 512, "bf16").saved_bytes(0) == 0
 
 
