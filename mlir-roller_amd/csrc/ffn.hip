@@ -10,8 +10,8 @@
 // the next product's matrix instructions read that type; everything else between the inputs and the outputs
 // is fp32, g and u included, which the forward pass keeps for the backward pass.
 //
-// With few tokens (up to 64) both forward products read the weights once and do little else; they take the
-// few_rows kernel instead of the tile engine.
+// With up to 16 tokens the forward pass does little but read the weights; it takes few_rows_kernel instead of
+// the tile engine, and with 16-bit types h stays in fp32 there (the second product splits it in two).
 #include "product_launch.h"
 #include "roller_ffn.h"
 
@@ -31,13 +31,15 @@ typedef bf16_t T;
 #endif
 
 constexpr int ES = sizeof(T), PER = 16 / ES;
-constexpr int FEW = 64;   // tokens up to which the forward products take the few_rows kernel
-constexpr int SPLIT_TOKENS = ES == 2 ? 16 : 0;   // tokens up to which h goes into the second product unrounded
+constexpr int FEW = 16;       // tokens up to which the forward products take few_rows_kernel,
+constexpr int FEW_ODD = 64;   // and with rows at odd places, which the tile engine would need packed copies of
+constexpr int EXACT_TOKENS = ES == 2 ? FEW : 0;   // tokens up to which h goes into the second product unrounded
 
 int pitch_of(int n) { return line_pitch(ES, n); }
 
-// The tile engine reads whole 16-byte chunks: a matrix whose rows are anything else is packed first.
-bool aligned(const FfnMatrix& m, int cols) { return (uintptr_t)m.p % 16 == 0 && m.ld % PER == 0 && cols % PER == 0; }
+// The tile engine loads dword-aligned rows; 16-bit rows at odd places are packed first, or with few tokens
+// multiplied by few_rows_kernel.
+bool aligned(const FfnMatrix& m) { return (uintptr_t)m.p % 4 == 0 && (long)m.ld * ES % 4 == 0; }
 
 class Carver {
  public:
@@ -54,9 +56,8 @@ class Carver {
   size_t used_ = 0;
 };
 
-// Space for a packed copy of m, if it needs one.
-T* pack_space(Carver& room, const FfnMatrix& m, int rows, int cols, bool need) {
-  (void)m;
+// Space for a packed copy, if one is needed.
+T* pack_space(Carver& room, int rows, int cols, bool need) {
   return need ? (T*)room.take((size_t)rows * pitch_of(cols) * ES) : nullptr;
 }
 
@@ -100,7 +101,8 @@ size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 struct ForwardRoom {
   T *x, *w_gate, *w_up, *w_down, *h;
   float* h32;
-  char* slabs;
+  char *arrivals, *pieces;
+  bool few;   // takes few_rows_kernel
   size_t bytes;
 };
 
@@ -108,36 +110,44 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
   Carver room(c.room);
   ForwardRoom r = {};
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
-  if (c.T <= SPLIT_TOKENS) r.h32 = (float*)room.take((size_t)c.T * s.pitch * 4);
-  else if (!c.saved) r.h = (T*)room.take((size_t)c.T * s.pitch * ES);
-  if (c.T > FEW) {
-    r.x = pack_space(room, c.x, c.T, c.D, unaligned || !aligned(c.x, c.D));
-    r.w_gate = pack_space(room, c.w_gate, c.F, c.D, unaligned || !aligned(c.w_gate, c.D));
-    r.w_up = pack_space(room, c.w_up, c.F, c.D, unaligned || !aligned(c.w_up, c.D));
-    r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
-    const size_t up = plan_product(ES, 1, 1, 0, c.T, s.cols, c.D, 1, c.compute_units).slab_bytes;
-    const size_t down = plan_product(ES, 0, 1, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes;
-    r.slabs = room.take(larger(up, down));
+  const bool odd = !aligned(c.x) || !aligned(c.w_gate) || !aligned(c.w_up) || !aligned(c.w_down);
+  r.few = c.T <= FEW || (c.T <= FEW_ODD && odd);
+  if (c.T <= EXACT_TOKENS) {
+    r.h32 = (float*)room.take((size_t)c.T * s.pitch * 4);
+  } else if (!c.saved) {
+    r.h = (T*)room.take((size_t)c.T * s.pitch * ES);
+  }
+  if (!r.few) {
+    const bool pack = c.T > FEW_ODD;
+    r.x = pack_space(room, c.T, c.D, pack && (unaligned || !aligned(c.x)));
+    r.w_gate = pack_space(room, c.F, c.D, pack && (unaligned || !aligned(c.w_gate)));
+    r.w_up = pack_space(room, c.F, c.D, pack && (unaligned || !aligned(c.w_up)));
+    r.w_down = pack_space(room, c.D, c.F, pack && (unaligned || !aligned(c.w_down)));
+    r.arrivals = room.take(kArrivalBytes);
+    const size_t up = plan_product(ES, 1, 1, 0, c.T, c.F, c.D, 1, c.compute_units, 0, kFewRowsTile + 1).piece_bytes;
+    const size_t down = plan_product(ES, 0, 1, 0, c.T, c.D, c.F, 1, c.compute_units, 0, kFewRowsTile + 1).piece_bytes;
+    r.pieces = room.take(larger(up, down));
   }
   r.bytes = room.used();
   return r;
 }
 
-template <int BLOCKS, int SPLIT, int KIND>
+template <int BLOCKS, int PARTS, int SPLIT, int KIND>
 int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated, const Store<T>& out, const FfnSaved& s) {
-  // Enough waves to keep the memory busy from every CU: up to 16 share the K of 16 weight rows, none with
-  // fewer than 256 bytes of each row.
+  // Enough waves to keep the memory busy from every CU: up to 16 share the K of a workgroup's rows, none with
+  // fewer than 256 bytes of each part of a row.
   auto waves = [&](int groups, int K) {
-    int w = 4;
-    while (w < 16 && (long)groups * w < 16L * c.compute_units && K * ES >= 512 * w) w *= 2;
+    int w = 1;
+    while (w < 16 && (long)groups * w < 16L * c.compute_units && K / PARTS * ES >= 512 * w) w *= 2;
     return 64 * w;
   };
+  constexpr int ROWS = 16 / PARTS;
   typedef typename x_type<T, SPLIT>::type H;
-  const int up = (s.cols + 15) / 16, down = (c.D + 15) / 16;
-  PT_TRY(launch(few_rows_kernel<T, BLOCKS, 1, 0, GatedForward<T, KIND>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
-                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, s.cols, c.D, gated));
-  return launch(few_rows_kernel<T, BLOCKS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
-                c.D, c.D, c.F, out);
+  const int up = (c.F + ROWS - 1) / ROWS, down = (c.D + ROWS - 1) / ROWS;
+  PT_TRY(launch(few_rows_kernel<T, BLOCKS, PARTS, 1, 0, GatedForward<T, KIND>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
+                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, c.D, gated));
+  return launch(few_rows_kernel<T, BLOCKS, PARTS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
+                c.D, c.F, out);
 }
 
 size_t forward_room(const FfnCall& c, bool unaligned) { return forward_carve(c, unaligned).bytes; }
@@ -147,28 +157,34 @@ int forward_as(const FfnCall& call) {
   FfnCall c = call;
   const ForwardRoom r = forward_carve(c, false);
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
-  T* h = c.saved ? (T*)((char*)c.saved + s.h) : r.h;
   GatedForward<T, KIND> gated = {};
-  gated.h = h;
-  gated.h32 = r.h32;
+  gated.h = c.saved ? (T*)((char*)c.saved + s.h) : r.h;
   gated.g = c.saved ? (float*)((char*)c.saved + s.g) : nullptr;
   gated.u = c.saved ? (float*)((char*)c.saved + s.u) : nullptr;
   gated.pitch = s.pitch;
   const Store<T> out = store(c.y, c.ldy, c.D);
-  if (c.T <= 16) return few_rows<1, SPLIT_TOKENS != 0>(c, r.h32 ? (const void*)r.h32 : h, gated, out, s);
-  if (c.T <= 32) return few_rows<2, 0>(c, h, gated, out, s);
-  if (c.T <= FEW) return few_rows<4, 0>(c, h, gated, out, s);
+  if (r.few) {
+    gated.h32 = r.h32;
+    constexpr int SPLIT = EXACT_TOKENS != 0;
+    const void* h = r.h32 ? (const void*)r.h32 : gated.h;
+    if (c.T <= 4) return few_rows<1, 4, SPLIT>(c, h, gated, out, s);
+    if (c.T <= 8) return few_rows<1, 2, SPLIT>(c, h, gated, out, s);
+    if (c.T <= 16) return few_rows<1, 1, SPLIT>(c, h, gated, out, s);
+    if (c.T <= 32) return few_rows<2, 1, 0>(c, h, gated, out, s);
+    return few_rows<4, 1, 0>(c, h, gated, out, s);
+  }
 
   PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
   PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
   PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
-  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, s.cols);
+  Arrivals arrivals = arrivals_at(r.arrivals, false);
+  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, c.F);
   up.b[1] = c.w_up.p;
   up.ldb1 = c.w_up.ld;
-  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: gate and up")));
-  const Problem down = problem(h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
-  return run_product<T, 1, 1, 0, 1, 0>(down, out, 1, r.slabs, c.stream, c.compute_units, "ffn: down");
+  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: gate and up")));
+  const Problem down = problem(gated.h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
+  return run_product<T, 1, 1, 0, 1, 0>(down, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: down");
 }
 
 int forward(const FfnCall& c) {
@@ -179,7 +195,7 @@ int forward(const FfnCall& c) {
 
 struct BackwardRoom {
   T *dy, *x, *w_gate, *w_up, *w_down, *dg, *du;
-  char* slabs;
+  char *arrivals, *pieces;
   size_t bytes;
 };
 
@@ -191,18 +207,19 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
   // (dg and du directly behind each other: the two batch entries of one product)
   r.dg = (T*)room.take(2 * n);
   r.du = r.dg ? r.dg + (size_t)c.T * s.pitch : nullptr;
-  r.dy = pack_space(room, c.dy, c.T, c.D, unaligned || !aligned(c.dy, c.D));
-  r.x = pack_space(room, c.x, c.T, c.D, unaligned || !aligned(c.x, c.D));
+  r.dy = pack_space(room, c.T, c.D, unaligned || !aligned(c.dy));
+  r.x = pack_space(room, c.T, c.D, unaligned || !aligned(c.x));
   // dx reads both weights with one leading dimension
-  const bool weights = unaligned || !aligned(c.w_gate, c.D) || !aligned(c.w_up, c.D) || c.w_gate.ld != c.w_up.ld;
-  r.w_gate = pack_space(room, c.w_gate, c.F, c.D, weights);
-  r.w_up = pack_space(room, c.w_up, c.F, c.D, weights);
-  r.w_down = pack_space(room, c.w_down, c.D, c.F, unaligned || !aligned(c.w_down, c.F));
-  size_t slabs = plan_product(ES, 0, 1, 0, c.T, s.cols, c.D, 1, c.compute_units).slab_bytes;
-  slabs = larger(slabs, plan_product(ES, 0, 2, 0, c.T, c.D, c.F, 1, c.compute_units).slab_bytes);
-  slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.F, c.D, c.T, 2, c.compute_units).slab_bytes);
-  slabs = larger(slabs, plan_product(ES, 0, 1, 0, c.D, c.F, c.T, 1, c.compute_units).slab_bytes);
-  r.slabs = room.take(slabs);
+  const bool weights = unaligned || !aligned(c.w_gate) || !aligned(c.w_up) || c.w_gate.ld != c.w_up.ld;
+  r.w_gate = pack_space(room, c.F, c.D, weights);
+  r.w_up = pack_space(room, c.F, c.D, weights);
+  r.w_down = pack_space(room, c.D, c.F, unaligned || !aligned(c.w_down));
+  r.arrivals = room.take(kArrivalBytes);
+  size_t pieces = plan_product(ES, 0, 1, 0, c.T, c.F, c.D, 1, c.compute_units).piece_bytes;
+  pieces = larger(pieces, plan_product(ES, 0, 2, 0, c.T, c.D, c.F, 1, c.compute_units).piece_bytes);
+  pieces = larger(pieces, plan_product(ES, 0, 1, 0, c.F, c.D, c.T, 2, c.compute_units).piece_bytes);
+  pieces = larger(pieces, plan_product(ES, 0, 1, 0, c.D, c.F, c.T, 1, c.compute_units).piece_bytes);
+  r.pieces = room.take(pieces);
   r.bytes = room.used();
   return r;
 }
@@ -214,14 +231,14 @@ int zero(void* p, int ld, int rows, int cols, hipStream_t stream) {
 }
 
 template <int KIND>
-int gated_backward(const FfnCall& c, const BackwardRoom& r, const FfnSaved& s, const Problem& dh) {
+int gated_backward(const FfnCall& c, const BackwardRoom& r, const FfnSaved& s, const Problem& dh, Arrivals& arrivals) {
   GatedBackward<T, KIND> gated = {};
   gated.g = (const float*)((char*)c.saved + s.g);
   gated.u = (const float*)((char*)c.saved + s.u);
   gated.dg = r.dg;
   gated.du = r.du;
   gated.pitch = s.pitch;
-  return run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.slabs, c.stream, c.compute_units, "ffn: dh");
+  return run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dh");
 }
 
 int backward(const FfnCall& call) {
@@ -235,18 +252,19 @@ int backward(const FfnCall& call) {
   const BackwardRoom r = backward_carve(c, false);
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
   const T* h = (const T*)((char*)c.saved + s.h);
+  Arrivals arrivals = arrivals_at(r.arrivals, false);
   PT_TRY(pack(c.dy, c.T, c.D, r.dy, c.stream));
   if (c.dw_down) {
     const Problem p = problem(c.dy.p, c.dy.ld, h, s.pitch, c.D, c.F, c.T, c.D, c.F);
-    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, store(c.dw_down, c.ld_dw_down, c.F), 1, r.slabs, c.stream, c.compute_units, "ffn: dw_down")));
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, store(c.dw_down, c.ld_dw_down, c.F), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_down")));
   }
   if (!c.dx && !c.dw_gate) return RL_OK;
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
-  const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, s.cols);
+  const Problem dh = problem(c.dy.p, c.dy.ld, c.w_down.p, c.w_down.ld, c.T, c.F, c.D, c.T, c.F);
   switch (c.activation) {
-    case ACT_SILU: PT_TRY(gated_backward<ACT_SILU>(c, r, s, dh)); break;
-    case ACT_GELU: PT_TRY(gated_backward<ACT_GELU>(c, r, s, dh)); break;
-    default: PT_TRY(gated_backward<ACT_GELU_TANH>(c, r, s, dh)); break;
+    case ACT_SILU: PT_TRY(gated_backward<ACT_SILU>(c, r, s, dh, arrivals)); break;
+    case ACT_GELU: PT_TRY(gated_backward<ACT_GELU>(c, r, s, dh, arrivals)); break;
+    default: PT_TRY(gated_backward<ACT_GELU_TANH>(c, r, s, dh, arrivals)); break;
   }
   if (c.dx) {
     PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
@@ -254,7 +272,7 @@ int backward(const FfnCall& call) {
     Problem p = problem(r.dg, s.pitch, c.w_gate.p, c.w_gate.ld, c.T, c.D, c.F, c.T, c.D);
     p.a[1] = r.du;
     p.b[1] = c.w_up.p;
-    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, store(c.dx, c.ld_dx, c.D), 1, r.slabs, c.stream, c.compute_units, "ffn: dx")));
+    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, store(c.dx, c.ld_dx, c.D), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
   }
   if (c.dw_gate) {
     PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
@@ -264,7 +282,7 @@ int backward(const FfnCall& call) {
     out.c[1] = (T*)c.dw_up;
     out.ldc1 = c.ld_dw_up;
     out.vec = out.vec && vec_ok(c.dw_up, c.ld_dw_up);
-    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, out, 2, r.slabs, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, out, 2, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
   }
   return RL_OK;
 }

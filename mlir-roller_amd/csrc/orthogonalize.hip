@@ -29,7 +29,9 @@ template <class Op> constexpr float kScale = sizeof(Op) == 2 ? 256.0f : 1.0f;
 constexpr int NORM_BLOCKS = 256;
 
 template <class T>
-__global__ __launch_bounds__(256) void norm_kernel(const T* G, int ld, long stride, int rows, int cols, double* partial) {
+__global__ __launch_bounds__(256) void norm_kernel(const T* G, int ld, long stride, int rows, int cols, double* partial, unsigned* clear, int n_clear) {
+  if (blockIdx.y == 0)   // the arrival counters of the first product
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_clear; i += gridDim.x * 256) clear[i] = 0;
   const T* g = G + blockIdx.y * stride;
   double sum = 0.0;   // (fp64: squares of entries beyond 1.8e19 overflow fp32)
   for (long r = blockIdx.x * 4L + threadIdx.x / 64; r < rows; r += gridDim.x * 4L)   // 64 lanes per row
@@ -131,7 +133,7 @@ struct Symmetric {
 template <class Op>
 struct Gram {
   Symmetric<Op> A;
-  __device__ __forceinline__ Gram at(int batch, int) const { return {A.of(batch)}; }
+  __device__ __forceinline__ Gram at(int batch) const { return {A.of(batch)}; }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
   __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const { A.put(m, n, v * (1.0f / (kScale<Op> * kScale<Op>)), ok); }
@@ -142,7 +144,7 @@ template <class Op>
 struct Polynomial {
   Symmetric<Op> A, B;
   float b, c;
-  __device__ __forceinline__ Polynomial at(int batch, int) const { return {A.of(batch), B.of(batch), b, c}; }
+  __device__ __forceinline__ Polynomial at(int batch) const { return {A.of(batch), B.of(batch), b, c}; }
   struct In {
     v4f ao, dn;
     float dm;
@@ -173,7 +175,7 @@ struct Update {
   T* out;         // NULL: X goes on
   int ldo, l, vec;
   long out_stride;
-  __device__ __forceinline__ Update at(int batch, int) const {
+  __device__ __forceinline__ Update at(int batch) const {
     Update o = *this;
     o.from += batch * stride;
     o.to += batch * stride;
@@ -215,7 +217,7 @@ struct Room {
   void *ao, *bo;
   float *da, *db;
   double* partial;
-  char* slabs;
+  char *arrivals, *pieces;
   int s, l;        // sides of X
   int l8, s8;      // the same up to whole chunks: columns written
   int pitch, sq;   // elements from row to row of X, and of A and B
@@ -253,12 +255,13 @@ Room carve(const OrthoCall& c) {
   r.da = (float*)take((size_t)c.batch * r.sq * 4);
   r.db = (float*)take((size_t)c.batch * r.sq * 4);
   r.partial = (double*)take((size_t)c.batch * NORM_BLOCKS * 8);
-  const size_t gram = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.l, c.batch, c.compute_units).slab_bytes;
-  const size_t poly = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.s, c.batch, c.compute_units).slab_bytes;
-  const size_t update = plan_product(sizeof(Op), 0, 1, 0, r.s, r.l8, r.s, c.batch, c.compute_units).slab_bytes;
-  size_t slabs = gram > poly ? gram : poly;
-  slabs = slabs > update ? slabs : update;
-  r.slabs = take(slabs);
+  const size_t gram = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.l, c.batch, c.compute_units).piece_bytes;
+  const size_t poly = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.s, c.batch, c.compute_units).piece_bytes;
+  const size_t update = plan_product(sizeof(Op), 0, 1, 0, r.s, r.l8, r.s, c.batch, c.compute_units).piece_bytes;
+  size_t pieces = gram > poly ? gram : poly;
+  pieces = pieces > update ? pieces : update;
+  r.arrivals = take(kArrivalBytes);
+  r.pieces = take(pieces);
   r.bytes = used;
   return r;
 }
@@ -268,8 +271,9 @@ int run(const OrthoCall& c) {
   const Room r = carve<Op>(c);
   const int tall = c.rows > c.cols;
   const long x_stride = (long)r.s * r.pitch;
+  Arrivals arrivals = arrivals_at(r.arrivals, true);   // (by norm_kernel)
   const int blocks = c.rows < 4 * NORM_BLOCKS ? (c.rows + 3) / 4 : NORM_BLOCKS;
-  PT_TRY(launch(norm_kernel<T>, "orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial));
+  PT_TRY(launch(norm_kernel<T>, "orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial, arrivals.set[0], kMaxArrivals));
   PT_TRY(launch(first_kernel<T, Op>, "orthogonalize: first X", dim3((r.l8 + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
                 r.s, r.l, r.l8, r.pitch, x_stride, r.x[0], (Op*)r.op[0]));
   const int vec = (uintptr_t)c.o % (4 * sizeof(T)) == 0 && c.ldo % 4 == 0 && c.stride_o % 4 == 0;
@@ -286,12 +290,12 @@ int run(const OrthoCall& c) {
     p.K = r.l;
     p.batch_a = p.batch_b = x_stride;
     Symmetric<Op> A = {(Op*)r.ao, r.da, r.s8, r.sq}, B = {(Op*)r.bo, r.db, r.s8, r.sq};
-    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Gram<Op>{A}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: X X^T")));
+    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Gram<Op>{A}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: X X^T")));
     p.a[0] = p.b[0] = r.ao;
     p.lda = p.ldb = p.ldb1 = r.sq;
     p.K = r.s;
     p.batch_a = p.batch_b = (long)r.s8 * r.sq;
-    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Polynomial<Op>{A, B, b, cc}, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: A A")));
+    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Polynomial<Op>{A, B, b, cc}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: A A")));
     const int next = 1 - cur;
     Update<T, Op> u = {};
     u.from = sizeof(Op) == 2 ? r.x[0] : r.x[cur];
@@ -315,7 +319,7 @@ int run(const OrthoCall& c) {
     p.M_out = r.s;
     p.N_out = r.l8;
     p.batch_b = x_stride;
-    PT_TRY((run_product<Op, 1, 0, 0, 1, 0>(p, u, c.batch, r.slabs, c.stream, c.compute_units, "orthogonalize: B X")));
+    PT_TRY((run_product<Op, 1, 0, 0, 1, 0>(p, u, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: B X")));
     cur = next;
   }
   const float* x = sizeof(Op) == 2 ? r.x[0] : r.x[cur];

@@ -38,40 +38,73 @@ template <> struct tile<0> { static constexpr int BM = 256, BN = 256, WM = 128, 
 template <> struct tile<1> { static constexpr int BM = 192, BN = 192, WM = 96, WN = 96, PER_CU = 1, BUFS = 3; };
 template <> struct tile<2> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 1, BUFS = 4; };
 template <> struct tile<3> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 2, BUFS = 4; };
+template <> struct tile<4> { static constexpr int BM = 32, BN = 64, WM = 32, WN = 32, PER_CU = 3, BUFS = 4; };
 
 template <int K, class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
-int launch_tile(const Problem& p, const Partial& part, const Epi& epi, int batch, hipStream_t stream, const char* what) {
+int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream, const char* what) {
   typedef tile<K> t;
-  // a gated wave tile of 32 or 96 columns is 16 or 48 of each kind: blocks of 16
-  typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, (GATED && t::WN / 2 % 32 != 0) ? 16 : 32, t::BUFS> S;
+  // Blocks of 32 x 32, or of 16 x 16 where 32 do not fit: gated wave tiles of 32 or 96 columns are 16 or 48 of
+  // each kind, and the few-rows tile has two blocks of 16 rows.
+  constexpr int MI = K == kFewRowsTile || (GATED && t::WN / 2 % 32 != 0) ? 16 : 32;
+  typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, MI, t::BUFS> S;
+  static_assert(t::BM == kTiles[K].bm && t::BN == kTiles[K].bn, "the plan's tiles");
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits;
   if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
-  return launch(tile_kernel<S, Epi>, what, dim3((unsigned)groups, 1, batch), S::NT, stream, p, part, epi);
+  return launch(tile_kernel<S, Epi>, what, dim3((unsigned)groups, 1, batch), S::NT, stream, p, epi);
 }
 
-// The product `p` (extents, operands) with epilogue `epi`: tile and split by plan(), slabs of a split one
-// from `room` (plan().slab_bytes of it).
-template <class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
-int run_product(Problem p, const Epi& epi, int batch, void* room, hipStream_t stream, int compute_units, const char* what) {
-  const Plan plan = plan_product(sizeof(T), GATED, SEGS, SYM, p.M_out, p.N_out, p.K, batch, compute_units);
+// Arrival counters of the products of one call, in its workspace: two sets that take turns.  Every product
+// clears the other set for the next one, whether it uses its own or not.  `ready`: the set whose turn it is
+// has been cleared, by the product before or by another kernel of the call; a first product that gains more
+// from splitting than that costs launches a kernel for it.
+struct Arrivals {
+  unsigned* set[2];
+  bool ready;
+  int turn = 0;
+};
+constexpr size_t kArrivalBytes = 2 * kMaxArrivals * sizeof(unsigned);
+inline Arrivals arrivals_at(void* room, bool ready) { return {{(unsigned*)room, (unsigned*)room + kMaxArrivals}, ready}; }
+
+// Which tiles a product may take: the few-rows tile exists for K-major operands.
+template <int A_KM, int B_KM, int SEGS, int SYM>
+constexpr int tiles_end() { return A_KM && B_KM && !SYM && SEGS == 1 ? kFewRowsTile + 1 : kFewRowsTile; }
+
+// Fills in p's split by `plan` and takes this product's turn of the arrival counters.
+inline int take_plan(Problem& p, const Plan& plan, void* room, Arrivals& arrivals, hipStream_t stream) {
   p.splits = plan.splits;
   p.steps_per_split = plan.steps_per_split;
-  Partial part = {};
-  part.slab = (float*)room;
-  part.pitch = (p.N_out + 3) / 4 * 4;
-  part.slab_size = (long)p.M_out * part.pitch;
-  part.per_split = batch * (GATED ? 2 : 1);
-  switch (plan.tile) {
-    case 0: PT_TRY((launch_tile<0, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
-    case 1: PT_TRY((launch_tile<1, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
-    case 2: PT_TRY((launch_tile<2, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
-    default: PT_TRY((launch_tile<3, T, A_KM, B_KM, GATED, SEGS, SYM>(p, part, epi, batch, stream, what))); break;
+  p.pieces = (float*)room;
+  p.arrivals = arrivals.set[arrivals.turn];
+  arrivals.turn ^= 1;
+  p.clear = arrivals.set[arrivals.turn];
+  p.n_clear = kMaxArrivals;
+  if (p.splits > 1 && !arrivals.ready)
+    PT_TRY(launch(zero_kernel<unsigned>, "clearing arrival counters", dim3(kMaxArrivals / 256), 256, stream, p.arrivals, kMaxArrivals, 1, kMaxArrivals));
+  arrivals.ready = true;
+  return RL_OK;
+}
+
+// The product `p` (extents, operands) with epilogue `epi`: tile and split by plan_product, pieces of split
+// tiles in `room` (piece_bytes of the plan).
+template <class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
+int run_product(Problem p, const Epi& epi, int batch, void* room, Arrivals& arrivals, hipStream_t stream, int compute_units, const char* what) {
+  constexpr int END = tiles_end<A_KM, B_KM, SEGS, SYM>();
+  Plan plan = plan_product(sizeof(T), GATED, SEGS, SYM, p.M_out, p.N_out, p.K, batch, compute_units, 0, END);
+  if (plan.splits > 1 && !arrivals.ready) {
+    const Plan whole = plan_product(sizeof(T), GATED, SEGS, SYM, p.M_out, p.N_out, p.K, batch, compute_units, 0, END, 1);
+    if (whole.time < plan.time + kClearLaunch) plan = whole;
   }
-  if (p.splits == 1) return RL_OK;
-  const long quads = (long)p.M_out * (part.pitch / 4);
-  return launch(join_kernel<Epi, GATED != 0>, what, dim3(blocks_for(quads), 1, batch), 256, stream, part, p.splits,
-                SYM ? kTiles[plan.tile].bm : 0, p.M_out, p.N_out, epi);
+  PT_TRY(take_plan(p, plan, room, arrivals, stream));
+  switch (plan.tile) {
+    case 0: return launch_tile<0, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+    case 1: return launch_tile<1, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+    case 2: return launch_tile<2, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+    case 3: return launch_tile<3, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+    default: break;
+  }
+  if constexpr (END > kFewRowsTile) return launch_tile<kFewRowsTile, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+  else return RL_OK;
 }
 
 }  // namespace product

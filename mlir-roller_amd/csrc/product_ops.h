@@ -1,7 +1,7 @@
 // What follows a product: the epilogues of the matrix-product engine (product_tile.h) for the gated
 // feed-forward block and for Newton-Schulz orthogonalisation, and the small kernels around them.
 //
-// An epilogue is a struct with at(batch, split), which picks the buffers of a batch entry, get(m, n), which
+// An epilogue is a struct with at(batch), which picks the buffers of a batch entry, get(m, n), which
 // loads what it needs besides the product, and put(m, n, v, in, ok): four consecutive columns n .. n+3 of row
 // m, n a multiple of 4 (gated products: put(m, n, gate, up, in, ok)), stored if ok.
 
@@ -81,7 +81,7 @@ struct Store {
   T* c[2];      // one per batch entry
   int ldc, ldc1, N;
   int vec;      // rows of 4 elements are aligned
-  __device__ __forceinline__ Store at(int batch, int) const {
+  __device__ __forceinline__ Store at(int batch) const {
     Store o = *this;
     if (batch) {
       o.c[0] = c[1];
@@ -112,7 +112,7 @@ struct GatedForward {
   float* h32;     // h unrounded, NULL: not needed
   float *g, *u;   // NULL: not kept
   int pitch;
-  __device__ __forceinline__ GatedForward at(int, int) const { return *this; }
+  __device__ __forceinline__ GatedForward at(int) const { return *this; }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
   __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up, In, bool ok) const {
@@ -136,7 +136,7 @@ struct GatedBackward {
   const float *g, *u;
   T *dg, *du;
   int pitch;
-  __device__ __forceinline__ GatedBackward at(int, int) const { return *this; }
+  __device__ __forceinline__ GatedBackward at(int) const { return *this; }
   struct In {
     v4f gate, up;
   };
@@ -162,35 +162,8 @@ struct GatedBackward {
 
 // ---- small kernels ----------------------------------------------------------------------------------
 
-// Sums the slabs of a split product in split order and hands them to the epilogue.  `tile`: the product is
-// symmetric and has no tiles of that size above its diagonal, where the mirror image is taken.
-template <class Epi, bool TWO>
-__global__ __launch_bounds__(256) void join_kernel(const Partial part, int splits, int tile, int M_out, int N_out, const Epi epi) {
-  const int quads = (N_out + 3) / 4;
-  const auto out = epi.at(blockIdx.z, 0);
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)M_out * quads; i += gridDim.x * 256L) {
-    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
-    const float* p = part.slab + (long)blockIdx.z * part.slab_size;
-    v4f v = {0.0f, 0.0f, 0.0f, 0.0f}, w = v;
-    const bool above = tile && n / tile > m / tile;
-    for (int s = 0; s < splits; ++s) {
-      if (above) {
-        const float* q = p + (long)n * part.pitch + m;
-        v += v4f{q[0], q[part.pitch], q[2L * part.pitch], q[3L * part.pitch]};
-      } else {
-        const float* q = p + (long)m * part.pitch + n;
-        v += *(const v4f*)q;
-        if constexpr (TWO) w += *(const v4f*)(q + part.slab_size);
-      }
-      p += part.per_split * part.slab_size;
-    }
-    if constexpr (TWO) out.put(m, n, v, w, out.get(m, n), true);
-    else out.put(m, n, v, out.get(m, n), true);
-  }
-}
-
-// Copies a matrix whose rows are not whole aligned 16-byte chunks into one whose rows are, with zeros
-// behind each row's end.  One element per access: such rows may start at any address.
+// Copies a matrix whose rows are not dword-aligned (16-bit elements at odd places) into one whose rows are,
+// with zeros up to a whole chunk.  One element per access: such rows may start at any address.
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* src, int ld, int rows, int cols, T* dst, int pitch) {
   constexpr int PER = 16 / sizeof(T);
@@ -208,16 +181,23 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int ld, int row
 // rows x cols zeros (the gradient of a weight over no tokens).
 template <class T>
 __global__ __launch_bounds__(256) void zero_kernel(T* c, int ld, int rows, int cols) {
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * cols; i += gridDim.x * 256L) c[i / cols * ld + i % cols] = (T)0.0f;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * cols; i += gridDim.x * 256L) c[i / cols * ld + i % cols] = (T)0;
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------
-// A product with at most 16 * BLOCKS rows of x, bound by reading the weights once.  A workgroup owns 16
-// weight rows (GATED: 16 gate rows and the same 16 up rows) and its waves share out K, 128 bytes of each
-// row at a time; weights go from memory straight into the MFMA's registers (row lane % 16, 16-byte chunk
-// lane / 16 of each 64 bytes), many loads in flight per wave, no LDS until the waves' sums are added up.
-// Rows of x and of the weights may start at any element: a chunk is loaded whole, at the alignment of
-// its type, and the last one of a row element by element.
+// A product with at most 16 * BLOCKS rows of x, whose time is that of reading the weights once.  A workgroup owns
+// ROWS = 16 / PARTS weight rows (GATED: as many gate and up rows) and its waves share out K; weights go from
+// memory straight into the MFMA's registers, so that all of a small problem's bytes can be asked for at once
+// (the tile engine has at most three K steps on their way: with one token and weights 4096 x 1024 it took 8.6 us
+// for the gate and up product where this kernel takes 5.8); no LDS until the waves' sums are added up.
+//
+// PARTS = 2 or 4: with few tokens the 16 x 16 block of an MFMA holds that many parts of K side by side, part q in
+// rows and columns 16 / PARTS * q and on; of the products of all parts with all parts only the diagonal blocks
+// are used.  A workgroup then owns fewer weight rows, and there are more of them (1024 rows: 64 workgroups of
+// 16 rows for 256 CUs, or 256 of 4: 8.9 us against PARTS_US us).
+//
+// Rows may start at any element: a chunk is loaded whole, at the alignment of its type, and the last one of a
+// row element by element.
 template <class T>
 PT_DEV v4u whole_chunk(const T* at) {
   v4u v;
@@ -257,17 +237,23 @@ PT_DEV void split_chunk(const float* x, v4u& hi, v4u& lo) {
   lo = __builtin_bit_cast(v4u, l);
 }
 
-template <class T, int BLOCKS, int GATED, int SPLIT, class Epi>
-__global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T, SPLIT>::type* x, int ldx, const T* w0, int ldw0, const T* w1, int ldw1, int M, int N, int N_out, int K, const Epi epi) {
-  constexpr int PER = 16 / sizeof(T), W = GATED ? 2 : 1, UNROLL = BLOCKS == 1 ? 8 : BLOCKS == 2 ? 4 : 2;
+template <class T, int BLOCKS, int PARTS, int GATED, int SPLIT, class Epi>
+__global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T, SPLIT>::type* x, int ldx, const T* w0, int ldw0, const T* w1, int ldw1, int M, int N, int K, const Epi epi) {
+  static_assert(PARTS == 1 || BLOCKS == 1, "parts share one block");
+  constexpr int PER = 16 / sizeof(T), W = GATED ? 2 : 1, UNROLL = BLOCKS == 1 ? 8 : BLOCKS == 2 ? 4 : 2, ROWS = 16 / PARTS;
   const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lr = lane & 15, lg = lane >> 4;
-  const int n0 = blockIdx.x * 16, row = n0 + lr < N ? n0 + lr : N - 1;   // (a row past the end is not stored)
+  const int part_k = (K + PARTS * 4 * PER - 1) / (PARTS * 4 * PER) * (4 * PER);   // whole loads
+  const int from = lr / ROWS * part_k, end = from + part_k < K ? from + part_k : K;
+  const int n0 = blockIdx.x * ROWS, row = n0 + lr % ROWS < N ? n0 + lr % ROWS : N - 1;   // (a row past the end is not stored)
   const T* wr[2] = {w0 + (long)row * ldw0, GATED ? w1 + (long)row * ldw1 : nullptr};
   typedef typename x_type<T, SPLIT>::type X;
   const X* xr[BLOCKS];
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b) xr[b] = x + (long)(16 * b + lr < M ? 16 * b + lr : M - 1) * ldx;
+  for (int b = 0; b < BLOCKS; ++b) {
+    const int m = 16 * b + lr % ROWS;
+    xr[b] = x + (long)(m < M ? m : M - 1) * ldx;
+  }
 
   v4f acc[W][BLOCKS];
 #pragma unroll
@@ -275,20 +261,20 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) acc[w][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // the waves take turns at groups of UNROLL x 64 bytes of k
+  // the waves take turns at groups of UNROLL x 64 bytes of every part
   constexpr int GROUP = UNROLL * 4 * PER, XV = SPLIT ? 2 : 1;   // XV: 16-byte loads per chunk of x
-  for (int k0 = wave * GROUP; k0 < K; k0 += waves * GROUP) {
+  for (int k0 = wave * GROUP; k0 < part_k; k0 += waves * GROUP) {
     v4u wv[W][UNROLL], xv[BLOCKS][UNROLL][XV];
-    const bool whole = k0 + GROUP <= K;
+    const bool whole = k0 + GROUP <= part_k && (PARTS - 1) * part_k + k0 + GROUP <= K;
 #pragma unroll
     for (int t = 0; t < UNROLL; ++t) {
-      const int k = k0 + (t * 4 + lg) * PER;
+      const int k = from + k0 + (t * 4 + lg) * PER;
 #pragma unroll
-      for (int w = 0; w < W; ++w) wv[w][t] = whole ? whole_chunk(wr[w] + k) : chunk_at(wr[w], k, K);
+      for (int w = 0; w < W; ++w) wv[w][t] = whole ? whole_chunk(wr[w] + k) : chunk_at(wr[w], k, end);
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-        for (int v = 0; v < XV; ++v) xv[b][t][v] = whole ? whole_chunk(xr[b] + k + 4 * v) : chunk_at(xr[b], k + 4 * v, K);
+        for (int v = 0; v < XV; ++v) xv[b][t][v] = whole ? whole_chunk(xr[b] + k + 4 * v) : chunk_at(xr[b], k + 4 * v, end);
     }
 #pragma unroll
     for (int t = 0; t < UNROLL; ++t)
@@ -309,38 +295,32 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
       }
   }
 
-  // the waves' sums, added in wave order
-  __shared__ v4f sums[16 * 64];
-  const auto out = epi.at(0, 0);
-  v4f total[W][BLOCKS];
-#pragma unroll
-  for (int w = 0; w < W; ++w)
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
-      __syncthreads();
-      sums[wave * 64 + lane] = acc[w][b];
-      __syncthreads();
-      if (wave == 0) {
-        v4f v = sums[lane];
-        for (int s = 1; s < waves; ++s) v += sums[s * 64 + lane];
-        total[w][b] = v;
-      }
-    }
-  if (wave != 0) return;
-  const int n = n0 + 4 * lg;
+  // the waves' sums, added in wave order, and the parts' in part order, by wave b for block b
+  __shared__ v4f sums[W][16][64];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {
-    const int m = 16 * b + lr;
-    if (m >= M || n >= N_out) continue;
-    // columns past the last weight row: zeros (padding of h), or not stored
-    if constexpr (GATED) {
-      v4f g = total[0][b], u = total[W - 1][b];
+    if (b) __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e >= N) g[e] = u[e] = 0.0f;
-      out.put(m, n, g, u, out.get(m, n), true);
+    for (int w = 0; w < W; ++w) sums[w][wave][lane] = acc[w][b];
+    __syncthreads();
+    if (wave != 0 || lane >= 64 / (PARTS * PARTS)) continue;
+    // lane of part 0 that holds columns 4 * quad .. of row m
+    const int quad = PARTS == 1 ? lane >> 4 : PARTS == 2 ? lane >> 3 : 0, m = 16 * b + lane % ROWS, n = n0 + 4 * quad;
+    v4f total[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      total[w] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < waves; ++s)
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) total[w] += sums[w][s][16 * (ROWS / 4 * q + quad) + ROWS * q + lane % ROWS];
+    }
+    if (m >= M || n >= N) continue;
+    // (columns past the last weight row hold copies of its products: padding of h, or not stored)
+    const auto out = epi.at(0);
+    if constexpr (GATED) {
+      out.put(m, n, total[0], total[W - 1], out.get(m, n), true);
     } else {
-      out.put(m, n, total[0][b], out.get(m, n), true);
+      out.put(m, n, total[0], out.get(m, n), true);
     }
   }
 }

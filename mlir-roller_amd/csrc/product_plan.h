@@ -20,48 +20,52 @@ struct TileCost {
   float step32, fixed32, once32;   // 32-bit operands
 };
 
+constexpr int kFewRowsTile = 4;   // for products of K-major operands only
 constexpr TileCost kTiles[] = {
     {256, 256, 0.967f, 9.5f, 0.0f, 6.886f, 10.0f, 0.0f},
     {192, 192, 0.554f, 7.6f, 0.0f, 3.872f, 7.8f, 0.0f},
     {128, 128, 0.316f, 4.6f, 0.3f, 1.740f, 4.9f, 0.0f},
     {64, 64, 0.159f, 1.0f, 2.8f, 0.448f, 1.2f, 2.4f},
+    {32, 64, 0.120f, 1.0f, 2.6f, 0.420f, 1.2f, 2.4f},
 };
-constexpr float kJoinFixed = 4.5f;          // the launch that adds up a split product, microseconds
-constexpr float kSlabBytes = 3.5e6f;        // bytes of slabs written or read per microsecond
+constexpr float kJoinFixed = 2.0f;          // what splitting a tile costs the one that adds it up, microseconds
+constexpr float kPieceBytes = 3.5e6f;       // bytes of pieces written or read per microsecond
+constexpr float kClearLaunch = 3.0f;        // a launch that clears the arrival counters, where no other does
 constexpr int kMaxSplits = 16;
-constexpr size_t kMaxSlabs = (size_t)1 << 29;
+constexpr int kMaxArrivals = 4096;          // tiles of a split product
+constexpr size_t kMaxPieces = (size_t)1 << 29;
 
 struct Plan {
+  float time;   // microseconds, by the model
   int tile, splits, steps_per_split;
-  size_t slab_bytes;
+  size_t piece_bytes;
 };
 
-inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out, int N_out, int K, int batch, int compute_units) {
+inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out, int N_out, int K, int batch, int compute_units, int first_tile = 0, int tiles_end = kFewRowsTile, int max_splits = kMaxSplits) {
   Plan best = {};
-  float best_time = 0.0f;
   const int kstep = 128 / elem_bytes;
   const int steps = (K + kstep - 1) / kstep * segs;
-  for (int t = 0; t < (int)(sizeof kTiles / sizeof kTiles[0]); ++t) {
+  for (int t = first_tile; t < tiles_end; ++t) {
     const TileCost& c = kTiles[t];
     const int out_n = gated ? c.bn / 2 : c.bn;
     const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + out_n - 1) / out_n;
     const long tiles = (sym ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch;
     const float step = elem_bytes == 2 ? c.step16 : c.step32, fixed = elem_bytes == 2 ? c.fixed16 : c.fixed32, once = elem_bytes == 2 ? c.once16 : c.once32;
-    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+    for (int splits = 1; splits <= max_splits; splits *= 2) {
       const int per = (steps + splits - 1) / splits;
-      // (every split has a step of its own, and two at least are worth a launch)
-      if (splits > 1 && (per < 2 || (long)(splits - 1) * per >= steps)) break;
-      const size_t slab = splits > 1 ? (size_t)splits * batch * (gated ? 2 : 1) * M_out * ((N_out + 3) / 4 * 4) * 4 : 0;
-      if (slab > kMaxSlabs) break;
+      // (every split has two steps at least; the largest tile is not split)
+      if (splits > 1 && (t == 0 || per < 2 || (long)(splits - 1) * per >= steps)) break;
+      const size_t pieces = splits > 1 ? (size_t)tiles * splits * c.bm * c.bn * 4 : 0;
+      if (splits > 1 && (pieces > kMaxPieces || tiles > kMaxArrivals)) break;
       const long per_cu = (tiles * splits + compute_units - 1) / compute_units;
       float time = once + per_cu * (per * step + fixed);
-      if (splits > 1) time += kJoinFixed + 2.0f * slab / kSlabBytes;
-      if (best_time == 0.0f || time < best_time) {
-        best_time = time;
+      if (splits > 1) time += kJoinFixed + 2.0f * pieces / kPieceBytes;
+      if (best.time == 0.0f || time < best.time) {
+        best.time = time;
         best.tile = t;
         best.splits = splits;
         best.steps_per_split = per;
-        best.slab_bytes = slab;
+        best.piece_bytes = pieces;
       }
     }
   }

@@ -57,11 +57,13 @@ struct int_c {
   static constexpr int value = V;
 };
 
-// Buffer resource over the 2 GiB from p, or over nothing: then a load returns 0 and touches no memory.
-PT_DEV v4u resource(const void* p, bool live) {
+// Buffer resource over `bytes` from p, or over nothing: a load beyond it returns 0 and touches no memory.
+PT_DEV v4u resource(const void* p, bool live, unsigned bytes) {
   const unsigned long at = (unsigned long)p;
-  return v4u{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, live ? 0x7fffffffu : 0u, 0x00020000u};
+  return v4u{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, live ? bytes : 0u, 0x00020000u};
 }
+// What is left of a matrix, in whole dwords, 2 GiB at most.
+PT_DEV unsigned dwords_of(long bytes) { return bytes > 0x7ffffffcL ? 0x7ffffffcu : ((unsigned)bytes + 3u) & ~3u; }
 
 #if __HIP_DEVICE_COMPILE__
 // 16 bytes per lane from `off` of the resource to LDS, lane by lane from `lds_at` on.  Written out, because
@@ -176,10 +178,16 @@ struct Problem {
   const void* b[3];   // one per K segment; GATED: gate and up weights of the one segment
   int lda, ldb, ldb1; // (ldb1: leading dimension of the up weights)
   int M, N, K;        // GATED: N counts columns of the product, each made of a gate and an up column
-  int M_out, N_out;   // rows and columns handed to the epilogue (those beyond M and N are zeros: the padding
-                      // of a buffer that a later product reads as K-major)
+  int M_out, N_out;   // rows and columns handed to the epilogue (those beyond M and N are zeros)
   long batch_a, batch_b;
-  int splits, steps_per_split;   // workgroups that share a tile's K steps, and how many each takes
+  // A tile's K steps may be shared out over workgroups.  Each then leaves its accumulators in `pieces`,
+  // and the one that finds the tile's arrival counter at splits - 1 adds them up in split order, whoever
+  // that is, so results do not depend on timing.  `arrivals` is zero when the launch starts; the launch
+  // before it on the stream sees to that (clear, n_clear).
+  int splits, steps_per_split;
+  float* pieces;
+  unsigned *arrivals, *clear;
+  int n_clear;
 };
 
 // Tile shape, operand forms and options of one kernel.
@@ -204,6 +212,7 @@ struct Shape {
   static constexpr int A_BYTES = BM * STEP_BYTES, B_BYTES = BN * STEP_BYTES;
   static constexpr int BUFS = BUFS_, LDS_BYTES = BUFS * (A_BYTES + B_BYTES);
   static constexpr int A_LOADS = BM * 8 / NT, B_LOADS = BN * 8 / NT;
+  static constexpr bool SPLIT = BM * BN <= 192 * 192;   // K steps may be shared out (the registers of 256 x 256 leave no room to)
   static constexpr int OUT_N = GATED ? BN / 2 : BN;   // result columns per tile
   static_assert(BM % WM == 0 && BN % WN == 0 && WM % MI == 0 && WN % MI == 0, "tile");
   static_assert((BM * 8) % NT == 0 && (BN * 8) % NT == 0, "whole loads per thread");
@@ -256,30 +265,12 @@ PT_DEV void triangle_tile(int p, int n, int& tm, int& tn) {
   tn = GROUP * g + p;
 }
 
-// Part of a split product: fp32, one slab of rows x pitch per split and batch entry (GATED: two, gate and up).
-struct Partial {
-  float* slab;
-  int pitch;
-  long slab_size;   // rows * pitch
-  int per_split;    // slabs per split
-  __device__ __forceinline__ Partial at(int batch, int split) const {
-    Partial o = *this;
-    o.slab += ((long)split * per_split + batch) * slab_size;
-    return o;
-  }
-  struct In {};
-  __device__ __forceinline__ In get(int, int) const { return {}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const {
-    if (ok) *(v4f*)(slab + (long)m * pitch + n) = v;
-  }
-  __device__ __forceinline__ void put(int m, int n, v4f gate, v4f up, In in, bool ok) const {
-    put(m, n, gate, in, ok);
-    if (ok) *(v4f*)(slab + slab_size + (long)m * pitch + n) = up;
-  }
-};
+// Cache policy of the pieces of a split tile: sc0 and sc1, coherent across the device's L2 caches, so that
+// neither side writes back or invalidates a cache that holds the operands.
+constexpr int COHERENT = 0x11;
 
 template <class S, class Epi>
-__global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S::WAVES / 4 : 1) void tile_kernel(const Problem p, const Partial partial, const Epi epi) {
+__global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S::WAVES / 4 : 1) void tile_kernel(const Problem p, const Epi epi) {
 #if __HIP_DEVICE_COMPILE__   // (the host pass needs the kernel's name only)
   typedef typename S::T T;
   constexpr int ES = S::ES, TM = S::TM, TN = S::TN, NT = S::NT;
@@ -304,6 +295,9 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   }
   const int m0 = tile_m * S::BM, n0 = tile_n * S::OUT_N;
   const int batch = blockIdx.z;
+
+  if (batch == 0)
+    for (int i = blockIdx.x * NT + tid; i < p.n_clear; i += gridDim.x * NT) p.clear[i] = 0;
 
   // K steps of this workgroup.  A segment is a whole number of steps: its last step is cut by K.
   const int seg_steps = (p.K + S::KSTEP - 1) / S::KSTEP;
@@ -357,12 +351,18 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   const long a_step = S::A_KM ? S::KSTEP : (long)S::KSTEP * p.lda;   // elements per K step
   const long b_step = S::B_KM ? S::KSTEP : (long)S::KSTEP * p.ldb;
 
-  // Operand bases of K step kt (of this workgroup).  A step at or beyond KT gets empty resources.
+  // bytes from the tile's first element to the matrix's end
+  const long a_end = ((S::A_KM ? (long)(p.M - 1 - m0) * p.lda + p.K : (long)(p.K - 1) * p.lda + p.M - m0)) * ES;
+  const long b_end = ((S::B_KM ? (long)(p.N - 1 - n0) * p.ldb + p.K : (long)(p.K - 1) * p.ldb + p.N - n0)) * ES;
+
+  // Operand bases of K step kt (of this workgroup).  A step at or beyond KT gets empty resources.  KTEST: the
+  // step may be the last, in which a chunk can reach past the matrix's last element.
   struct source {
     v4u a, b, b1;   // (b1: the up weights)
     int k_left;     // of K, from the step's first k on
   };
-  auto source_of = [&](int kt) __attribute__((always_inline)) {
+  auto source_of = [&](auto ktest, int kt) __attribute__((always_inline)) {
+    constexpr bool KTEST = decltype(ktest)::value;
     const bool live = kt < KT;
     int step = first_step + (live ? kt : 0), seg = 0;
     if constexpr (S::SEGS > 1) {
@@ -374,9 +374,9 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     const T* ap = (const T*)(S::SEGS > 1 && seg == 1 ? p.a[1] : S::SEGS > 2 && seg == 2 ? p.a[2] : p.a[0]) + a_tile + step * a_step;
     const T* bp = (const T*)(S::SEGS > 1 && seg == 1 ? p.b[1] : S::SEGS > 2 && seg == 2 ? p.b[2] : p.b[0]) + b_tile + step * b_step;
     source s;
-    s.a = resource(ap, live);
-    s.b = resource(bp, live);
-    if constexpr (S::GATED) s.b1 = resource((const T*)p.b[1] + b_tile1 + step * S::KSTEP, live);
+    s.a = resource(ap, live, KTEST ? dwords_of(a_end - step * a_step * ES) : 0x7fffffffu);
+    s.b = resource(bp, live, KTEST ? dwords_of(b_end - step * b_step * ES) : 0x7fffffffu);
+    if constexpr (S::GATED) s.b1 = resource((const T*)p.b[1] + b_tile1 + step * S::KSTEP, live, KTEST ? dwords_of(((long)(p.N - 1 - n0) * p.ldb1 + p.K - step * S::KSTEP) * ES) : 0x7fffffffu);
     s.k_left = p.K - step * S::KSTEP;
     return s;
   };
@@ -463,6 +463,8 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
 #pragma unroll
       for (int r = 0; r < REGS; ++r) acc[i][j][r] = 0.0f;
 
+  auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+
   // ---- K loop ----
   // A step is ROUNDS rounds of G slots; a round multiplies one set of fragments while the next set is read.
   // Buffer `cur` holds step kt, and the steps up to kt + BUFS - 1 are on their way into the others: of the
@@ -482,26 +484,49 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       acc[i][j] = mma<T, MI>::part(e / G, f.b[j], f.a[i], acc[i][j]);
     }
   };
-  auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+  // The steps that K cuts short are the last ones of the segments.  Where K ends inside a chunk of a K-major
+  // operand, what the chunk brought from behind K (the next row's first elements, or nobody's) is overwritten
+  // with zeros in LDS once it has landed.
+  constexpr int PER = 16 / ES;
+  const bool whole = p.K % S::KSTEP == 0 && (S::A_KM || p.M % PER == 0) && (S::B_KM || p.N % PER == 0);
+  const bool ragged = p.K % PER != 0;
+  auto is_cut = [&](int kt) __attribute__((always_inline)) { return kt < KT && (first_step + kt + 1) % seg_steps == 0; };
+  auto zero_tails = [&](int buf) __attribute__((always_inline)) {
+    const int left = p.K % S::KSTEP;
+    if (a_k < left && a_k + PER > left) {
+      if constexpr (S::A_KM) {
+#pragma unroll 1
+        for (int i = 0; i < S::A_LOADS; ++i)
+          for (int e = left - a_k; e < PER; ++e) lds_write<T>(buf * S::A_BYTES + (tid + i * NT) * 16 + e * ES, (T)0.0f);
+      }
+      if constexpr (S::B_KM) {
+#pragma unroll 1
+        for (int i = 0; i < S::B_LOADS; ++i)
+          for (int e = left - a_k; e < PER; ++e) lds_write<T>(BUFS * S::A_BYTES + buf * S::B_BYTES + (tid + i * NT) * 16 + e * ES, (T)0.0f);
+      }
+    }
+    __syncthreads();
+  };
   if (KT > 0) {
     frags f[2];
     {
 #pragma unroll
       for (int b = 0; b < BUFS; ++b) {
-        const source s = source_of(b);
+        const source s = source_of(int_c<1>{}, b);
 #pragma unroll
         for (int i = 0; i < (b + 1 < BUFS ? L : TAIL); ++i) load(int_c<1>{}, s, b, i);
       }
     }
     wait_loads((BUFS - 2) * L + TAIL);   // step 0 has landed
     __syncthreads();
+    if (ragged && is_cut(0)) zero_tails(0);
 #pragma unroll
     for (int i = 0; i < FRAGS; ++i) read(f[0], int_c<0>{}, int_c<0>{}, i);
     fence();
     auto step = [&](auto ktest, auto cur_c, int kt) __attribute__((always_inline)) {
       constexpr int cur = decltype(cur_c)::value;
       {
-        const source next = source_of(kt + BUFS - 1);
+        const source next = source_of(ktest, kt + BUFS - 1);
         constexpr int into = (cur + BUFS - 1) % BUFS;
         auto round = [&](auto round_c) __attribute__((always_inline)) {
           constexpr int r = decltype(round_c)::value;
@@ -530,8 +555,11 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       fence();
       wait_loads((BUFS - 2) * L);   // kt + 1 has landed
       __syncthreads();
+      if constexpr (decltype(ktest)::value) {
+        if (ragged && is_cut(kt + 1)) zero_tails((cur + 1) % BUFS);
+      }
       fence();
-      const source next = source_of(kt + BUFS);
+      const source next = source_of(ktest, kt + BUFS);
       constexpr int REST = G - EARLY;
 #pragma unroll
       for (int t = 0; t < REST; ++t) {
@@ -543,9 +571,9 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
         fence();
       }
     };
+    // Passes of BUFS steps: without the tests as long as the pass's loads and reads (up to step kt + 2 BUFS) stay
+    // clear of a cut step, with them around one.
     int kt = 0;
-    // steps none of whose loads (up to those of kt + BUFS) can be cut short by the end of K (of any segment)
-    const int cut_free = p.K % S::KSTEP == 0 ? KT : (S::SEGS > 1 ? 0 : (last_step == seg_steps ? KT - 1 - BUFS : KT));
     auto pass = [&](auto ktest) __attribute__((always_inline)) {
       step(ktest, int_c<0>{}, kt);
       step(ktest, int_c<1>{}, kt + 1);
@@ -553,8 +581,17 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       if constexpr (BUFS > 3) step(ktest, int_c<3 % BUFS>{}, kt + 3);
       kt += BUFS;
     };
-    while (kt + BUFS <= KT && kt + BUFS <= cut_free) pass(int_c<0>{});
-    while (kt + BUFS <= KT) pass(int_c<1>{});
+    if constexpr (S::SEGS == 1) {
+      const int free = whole ? KT : seg_steps - 1 - first_step - BUFS;   // passes that end at or before it
+      while (kt + BUFS <= KT && kt + BUFS <= free) pass(int_c<0>{});
+      while (kt + BUFS <= KT) pass(int_c<1>{});
+    } else {
+      for (int cut = seg_steps - 1 - first_step % seg_steps; kt + BUFS <= KT; cut += seg_steps) {
+        const int free = whole ? KT : cut - BUFS;
+        while (kt + BUFS <= KT && kt + BUFS <= free) pass(int_c<0>{});
+        while (kt + BUFS <= KT && kt <= cut) pass(int_c<1>{});
+      }
+    }
     if (kt < KT) step(int_c<1>{}, int_c<0>{}, kt);
     if constexpr (BUFS > 2) {
       if (kt + 1 < KT) step(int_c<1>{}, int_c<1>{}, kt + 1);
@@ -565,18 +602,64 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     wait_loads(0);   // the empty requests past the end have drained
   }
 
+  __syncthreads();   // the K loop is done with the LDS
+
+  // ---- a shared tile: leave the accumulators, and the last one in adds them up ----
+  if constexpr (S::SPLIT) if (p.splits > 1) {
+    constexpr int QUADS = REGS / 4;
+    const long tile = (long)batch * tiles + pid;
+    float* const pieces = p.pieces + tile * p.splits * (S::BM * S::BN);
+    {
+      const __amdgpu_buffer_rsrc_t mine = __builtin_amdgcn_make_buffer_rsrc(pieces + (long)split * (S::BM * S::BN), 0, S::BM * S::BN * 4, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]}), mine,
+                                                   (unsigned)((((i * TN + j) * QUADS + q) * NT + tid) * 16), 0, COHERENT);
+        fence();
+      }
+    }
+    wait_loads(0);   // (stores count as well: the piece has arrived in memory)
+    __syncthreads();
+    if (tid == 0) lds_write(0u, __hip_atomic_fetch_add(&p.arrivals[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(lds_read<unsigned>(0u)) != (unsigned)p.splits - 1) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      for (int s = 0; s < p.splits; ++s) {
+        const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(pieces + (long)s * (S::BM * S::BN), 0, S::BM * S::BN * 4, 0x00020000);
+        v4f v[TN][QUADS];
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q)
+            v[j][q] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, (unsigned)((((i * TN + j) * QUADS + q) * NT + tid) * 16), 0, COHERENT));
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = s == 0 ? v[j][q][e] : acc[i][j][4 * q + e] + v[j][q][e];
+      }
+      fence();
+    }
+  }
   // ---- every accumulator leaves once ----
   // Through LDS, which the K loop has left: each wave writes a row of its blocks there (its own part, so
   // no wave waits for another) and reads it back row by row, four columns a lane.  Stores and the
   // epilogue's own loads are then whole stretches of a row, and its code is a loop instead of a copy per
   // accumulator.  Rows are padded by 16 bytes: the 16-byte writes of the lanes of a block go to
   // consecutive rows.
-  __syncthreads();
   constexpr int PITCH = S::WN + 4;
   static_assert(S::WAVES * MI * PITCH * 4 <= S::LDS_BYTES, "a row of blocks per wave fits the LDS");
   const unsigned mine = wave * (MI * PITCH * 4);
   const unsigned to = mine + (lr * PITCH + 4 * lg) * 4;
-  auto leave = [&](auto out, auto mirror) __attribute__((always_inline)) {
+  const auto out = epi.at(batch);
+  {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -587,7 +670,7 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       const int mb = m0 + wm0 + i * MI;
       constexpr int COLS = S::GATED ? S::WN / 2 : S::WN, PER_ROW = COLS / 4, UNITS = MI * PER_ROW;   // 4 columns a unit
       const int nb = n0 + (S::GATED ? (wave % S::NWN) * (S::WN / 2) : wn0);
-      typedef typename decltype(out)::In In;
+      typedef typename Epi::In In;
       constexpr int PER_LANE = UNITS / 64, MOST = sizeof(In) > 32 ? 4 : 8;
       constexpr int BATCH = PER_LANE <= MOST ? PER_LANE : PER_LANE % MOST == 0 ? MOST : PER_LANE % 6 == 0 ? 6 : 4;
       static_assert(UNITS % 64 == 0 && PER_LANE % BATCH == 0, "whole batches");
@@ -622,15 +705,10 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       };
       units(int_c<0>{});
       // the mirror image of a tile below the diagonal: four rows of one column a unit
-      if constexpr (S::SYM && decltype(mirror)::value) {
+      if constexpr (S::SYM) {
         if (tile_m != tile_n) units(int_c<1>{});
       }
     }
-  };
-  if (p.splits > 1) {
-    leave(partial.at(batch, split), int_c<0>{});
-  } else {
-    leave(epi.at(batch, 0), int_c<1>{});
   }
 #endif
 }

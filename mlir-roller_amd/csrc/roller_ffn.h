@@ -28,14 +28,12 @@ struct FfnCall {
 
 // Bytes of the three kept buffers (h in the element type, g and u in fp32), each T x pitch.
 struct FfnSaved {
-  int cols;                // columns written: F, up to whole 16-byte chunks
   int pitch;               // elements from row to row
   size_t h, g, u, total;   // offsets
 };
 inline size_t ffn_round(size_t n) { return (n + 255) / 256 * 256; }
 inline FfnSaved ffn_saved(int es, int T, int F) {
   FfnSaved s;
-  s.cols = (F + 16 / es - 1) / (16 / es) * (16 / es);
   s.pitch = product::line_pitch(es, F);
   const size_t n = (size_t)T * s.pitch;
   s.h = 0;
