@@ -334,7 +334,7 @@ typedef struct rl_ortho_config {
 int rl_ortho_workspace_bytes(const rl_ortho_config* cfg, size_t* bytes);
 
 /* `coefficients`: host memory, (a, b, c) for each step, read before the call returns; NULL: 3.4445, -4.7750,
- * 2.0315 in every step.  They must keep |X| below 200 for bf16 matrices (operands are fp16 inside; any
+ * 2.0315 in every step.  They must keep |X| and |A| below 100 (operands are fp16 inside; any
  * schedule that converges stays below 2).  stride_g, stride_o: elements from one matrix of the stack to
  * the next. */
 int rl_orthogonalize(const rl_ortho_config* cfg, const float* coefficients, const void* G, int ldg, long stride_g, void* O,

@@ -5,14 +5,17 @@
 //
 // Precision.  The iteration multiplies the small directions of X by a (3.4 by default) in every step, and
 // with them the rounding errors of what is multiplied: with bf16 operands the result is 1 to 20 % off, in
-// 16-bit bf16 outputs that can hold 0.17 %.  So X is kept in fp32, and
-//   * bf16 matrices: the operands of the products are fp16 (11 bits instead of 8; |X| and |A| are bounded, so
-//     the range does not matter), and the diagonals of A and B, the one place where A and B are not small
-//     and whose errors add up along the rows of X, never pass through them:
+// 16-bit bf16 outputs that can hold 0.17 %.  So X is kept in fp32, and the operands of the products are fp16
+// (11 bits instead of 8; |X| and |A| are bounded, so the range does not matter):
+//   * The diagonals of A and B, the one place where they are not small and whose errors add up along the rows
+//     of X, never pass through 16 bits:
 //       (A^2)_ij = (Ao^2)_ij + (D_i + D_j) Ao_ij + [i = j] D_i^2      Ao = A without its diagonal D
 //       X <- (a + diag(B)) X + Bo X                                    Bo = B without its diagonal
-//     which leaves an error of 0.02 to 0.1 % of the norm, under the rounding of the output.
-//   * fp16 and fp32 matrices: the products run on fp32 operands.
+//   * bf16 matrices: one fp16 number per operand element, which leaves an error of 0.02 to 0.1 % of the norm,
+//     under the rounding of the output.
+//   * fp16 and fp32 matrices: two, high part and remainder (22 bits), and three of their four products,
+//     hi hi + hi lo + lo hi, as three segments of one K loop: an error of some 10^-7 of the norm, as with fp32
+//     products, at a third of the fp16 rate instead of a sixteenth.
 #include "product_launch.h"
 #include "roller_ortho.h"
 
@@ -20,9 +23,25 @@ namespace {
 
 using namespace product;
 
-// fp16 operands are scaled by 2^8: entries of a normalised X of n columns are around n^-1/2, and what is
-// below 2^-14 would lose bits as a subnormal.
-template <class Op> constexpr float kScale = sizeof(Op) == 2 ? 256.0f : 1.0f;
+// Operands are scaled by 2^9: entries of a normalised X of n columns are around n^-1/2, and what is below
+// 2^-14 (or a remainder below 2^-25) would lose bits as a subnormal.
+typedef half_t Op;
+constexpr float kScale = 512.0f, kUnscale = 1.0f / (kScale * kScale);
+
+// Writes four elements of an operand: to[0 ..], and with two parts the remainders `parts` elements further on.
+template <int PARTS>
+PT_DEV void put_operand(Op* to, long parts, v4f v) {
+  const v4f x = v * kScale;
+  const typename vec4<Op>::type hi = round4<Op>(x);
+  *(typename vec4<Op>::type*)to = hi;
+  if constexpr (PARTS == 2) store4(to + parts, v4f{x[0] - (float)hi[0], x[1] - (float)hi[1], x[2] - (float)hi[2], x[3] - (float)hi[3]});
+}
+template <int PARTS>
+PT_DEV v4f get_operand(const Op* at, long parts) {
+  v4f v = load4(at);
+  if constexpr (PARTS == 2) v += load4(at + parts);
+  return v * (1.0f / kScale);
+}
 
 // ---- norm and first X -------------------------------------------------------------------------------
 
@@ -49,10 +68,10 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* G, int ld, long stri
   if (threadIdx.x == 0) partial[blockIdx.y * gridDim.x + blockIdx.x] = sums[0];
 }
 
-// X0 in fp32 and as an operand, 64 x 64 elements per workgroup, transposed if G is tall; zeros behind the
-// rows' ends up to whole chunks.
-template <class T, class Op>
-__global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long stride, int tall, const double* partial, int n_partial, float eps, int s, int l, int l8, int pitch, long x_stride, float* X, Op* Xop) {
+// X0 in fp32 and as an operand, 64 x 64 elements per workgroup, transposed if G is tall; zeros behind
+// the ends of rows and columns up to whole patches.
+template <class T, int PARTS>
+__global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long stride, int tall, const double* partial, int n_partial, float eps, int s, int l, int pitch, long x_stride, float* X, Op* Xop, long parts) {
   __shared__ double total[256];
   __shared__ float patch[64][65];
   const int t = threadIdx.x;
@@ -74,12 +93,13 @@ __global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long str
   }
   for (int i = t / 64; i < 64; i += 4) {
     const int r = r0 + i, c = c0 + t % 64;
-    if (r >= s || c >= l8) continue;
-    float v = tall ? patch[i][t % 64] : c < l ? (float)g[(long)r * ld + c] : 0.0f;
+    float v = tall ? patch[i][t % 64] : c < l && r < s ? (float)g[(long)r * ld + c] : 0.0f;
     v = v / norm;
     const long at = blockIdx.z * x_stride + (long)r * pitch + c;
     X[at] = v;
-    if constexpr (sizeof(Op) == 2) Xop[at] = (Op)(v * kScale<Op>);
+    const Op hi = (Op)(v * kScale);
+    Xop[at] = hi;
+    if constexpr (PARTS == 2) Xop[parts + at] = (Op)(v * kScale - (float)hi);
   }
 }
 
@@ -105,13 +125,14 @@ __global__ __launch_bounds__(256) void out_kernel(const float* X, int s, int l, 
 
 // ---- epilogues --------------------------------------------------------------------------------------
 
-// Both halves of a symmetric matrix without its diagonal, and the diagonal: the buffers that one product
-// writes and the next ones read.
-template <class Op>
+// A symmetric matrix without its diagonal, and the diagonal: the buffers that one product writes and the next
+// ones read.
+template <int PARTS>
 struct Symmetric {
   Op* off;        // [rows][pitch]
   float* diag;    // [pitch]
   int rows, pitch;
+  long parts;     // from the high parts to the remainders
   __device__ __forceinline__ Symmetric of(int batch) const {
     Symmetric o = *this;
     o.off += (long)batch * rows * pitch;
@@ -123,63 +144,62 @@ struct Symmetric {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (ok && m == n + e) diag[m] = v[e];
-      x[e] = m == n + e ? 0.0f : v[e] * kScale<Op>;
+      x[e] = m == n + e ? 0.0f : v[e];
     }
-    if (ok) store4(off + (long)m * pitch + n, x);
+    if (ok) put_operand<PARTS>(off + (long)m * pitch + n, parts, x);
   }
 };
 
 // A = X X^T
-template <class Op>
+template <int PARTS>
 struct Gram {
-  Symmetric<Op> A;
+  Symmetric<PARTS> A;
   __device__ __forceinline__ Gram at(int batch) const { return {A.of(batch)}; }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const { A.put(m, n, v * (1.0f / (kScale<Op> * kScale<Op>)), ok); }
+  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const { A.put(m, n, v * kUnscale, ok); }
 };
 
 // B = b A + c A^2, from the product of Ao with itself
-template <class Op>
+template <int PARTS>
 struct Polynomial {
-  Symmetric<Op> A, B;
+  Symmetric<PARTS> A, B;
   float b, c;
   __device__ __forceinline__ Polynomial at(int batch) const { return {A.of(batch), B.of(batch), b, c}; }
   struct In {
     v4f ao, dn;
     float dm;
   };
-  __device__ __forceinline__ In get(int m, int n) const { return {load4(A.off + (long)m * A.pitch + n), *(const v4f*)(A.diag + n), A.diag[m]}; }
+  __device__ __forceinline__ In get(int m, int n) const { return {get_operand<PARTS>(A.off + (long)m * A.pitch + n, A.parts), *(const v4f*)(A.diag + n), A.diag[m]}; }
   __device__ __forceinline__ void put(int m, int n, v4f v, In in, bool ok) const {
-    const v4f ao = in.ao * (1.0f / kScale<Op>), dn = in.dn;
-    const float dm = in.dm;
     v4f x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float sq = v[e] * (1.0f / (kScale<Op> * kScale<Op>));
-      x[e] = m == n + e ? b * dm + c * (sq + dm * dm) : b * ao[e] + c * (sq + (dm + dn[e]) * ao[e]);
+      const float sq = v[e] * kUnscale;
+      x[e] = m == n + e ? b * in.dm + c * (sq + in.dm * in.dm) : b * in.ao[e] + c * (sq + (in.dm + in.dn[e]) * in.ao[e]);
     }
     B.put(m, n, x, ok);
   }
 };
 
-// X <- (a + diag(B)) X + Bo X; the last step of a wide matrix writes the output instead
-template <class T, class Op>
+// X <- (a + diag(B)) X + Bo X, in place (every element is read and written by one lane); the last step of a
+// wide matrix writes the output instead
+template <class T, int PARTS>
 struct Update {
-  const float *from, *diag;
-  float* to;
+  float* x;
+  const float* diag;
   Op* op;
+  long parts;
   int pitch, diag_pitch;
   long stride;
   float a, scale;
   T* out;         // NULL: X goes on
-  int ldo, l, vec;
+  int ldo, s, l, vec;
   long out_stride;
   __device__ __forceinline__ Update at(int batch) const {
     Update o = *this;
-    o.from += batch * stride;
-    o.to += batch * stride;
-    if (o.op) o.op += batch * stride;
+    o.x += batch * stride;
+    o.op += batch * stride;
     if (o.out) o.out += batch * out_stride;
     o.diag += (long)batch * diag_pitch;
     return o;
@@ -188,45 +208,52 @@ struct Update {
     v4f x;
     float d;
   };
-  __device__ __forceinline__ In get(int m, int n) const { return {*(const v4f*)(from + (long)m * pitch + n), diag[m]}; }
+  __device__ __forceinline__ In get(int m, int n) const { return {*(const v4f*)(x + (long)m * pitch + n), diag[m]}; }
   __device__ __forceinline__ void put(int m, int n, v4f v, In in, bool ok) const {
     const long i = (long)m * pitch + n;
-    const v4f x = in.x * (a + in.d) + v * (1.0f / (kScale<Op> * kScale<Op>));
+    const v4f y = in.x * (a + in.d) + v * kUnscale;
     if (!ok) return;
     if (out) {
+      if (m >= s) return;
       T* o = out + (long)m * ldo + n;
       if (vec && n + 3 < l) {
-        store4(o, x * scale);
+        store4(o, y * scale);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (n + e < l) o[e] = (T)(x[e] * scale);
+          if (n + e < l) o[e] = (T)(y[e] * scale);
       }
       return;
     }
-    *(v4f*)(to + i) = x;
-    if constexpr (sizeof(Op) == 2) store4(op + i, x * kScale<Op>);
+    *(v4f*)(x + i) = y;
+    put_operand<PARTS>(op + i, parts, y);
   }
 };
 
 // ---- host -------------------------------------------------------------------------------------------
 
 struct Room {
-  float* x[2];     // X in fp32 (fp32 operands: the two take turns; fp16: the first)
-  half_t* op[2];   // X as an operand, taking turns (fp16 operands)
-  void *ao, *bo;
+  float* x;        // X in fp32
+  Op* op[2];       // X as an operand, taking turns
+  Op *ao, *bo;
   float *da, *db;
   double* partial;
   char *arrivals, *pieces;
   int s, l;        // sides of X
-  int l8, s8;      // the same up to whole chunks: columns written
+  int l64, s64;    // the same up to whole K steps: rows and columns that exist, zeros beyond s and l
   int pitch, sq;   // elements from row to row of X, and of A and B
+  long x_parts, sq_parts;   // from the high parts of an operand to the remainders
   size_t bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-template <class Op>
+template <int PARTS>
+Plan plan_of(int sym, int M_out, int N_out, int K, const OrthoCall& c) {
+  return plan_product(sizeof(Op), 0, PARTS == 2 ? 3 : 1, sym, M_out, N_out, K, c.batch, c.compute_units, 0, sym || PARTS == 2 ? kFewRowsTile : tiles_end<1, 0, 1, 0>());
+}
+
+template <int PARTS>
 Room carve(const OrthoCall& c) {
   Room r = {};
   char* base = c.room;
@@ -238,26 +265,23 @@ Room carve(const OrthoCall& c) {
   };
   r.s = c.rows < c.cols ? c.rows : c.cols;
   r.l = c.rows < c.cols ? c.cols : c.rows;
-  r.l8 = (r.l + 7) / 8 * 8;
-  r.s8 = (r.s + 7) / 8 * 8;
+  r.l64 = (r.l + 63) / 64 * 64;
+  r.s64 = (r.s + 63) / 64 * 64;
   r.pitch = line_pitch(sizeof(Op), r.l);
   r.sq = line_pitch(sizeof(Op), r.s);
-  const size_t x = (size_t)c.batch * r.s * r.pitch, q = (size_t)c.batch * r.s8 * r.sq;
-  r.x[0] = (float*)take(x * 4);
-  if (sizeof(Op) == 2) {
-    r.op[0] = (half_t*)take(x * 2);
-    r.op[1] = (half_t*)take(x * 2);
-  } else {
-    r.x[1] = (float*)take(x * 4);
-  }
-  r.ao = take(q * sizeof(Op));
-  r.bo = take(q * sizeof(Op));
+  r.x_parts = (long)c.batch * r.s64 * r.pitch;
+  r.sq_parts = (long)c.batch * r.s64 * r.sq;
+  r.x = (float*)take((size_t)r.x_parts * 4);
+  r.op[0] = (Op*)take((size_t)r.x_parts * sizeof(Op) * PARTS);
+  r.op[1] = (Op*)take((size_t)r.x_parts * sizeof(Op) * PARTS);
+  r.ao = (Op*)take((size_t)r.sq_parts * sizeof(Op) * PARTS);
+  r.bo = (Op*)take((size_t)r.sq_parts * sizeof(Op) * PARTS);
   r.da = (float*)take((size_t)c.batch * r.sq * 4);
   r.db = (float*)take((size_t)c.batch * r.sq * 4);
   r.partial = (double*)take((size_t)c.batch * NORM_BLOCKS * 8);
-  const size_t gram = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.l, c.batch, c.compute_units).piece_bytes;
-  const size_t poly = plan_product(sizeof(Op), 0, 1, 1, r.s8, r.s8, r.s, c.batch, c.compute_units).piece_bytes;
-  const size_t update = plan_product(sizeof(Op), 0, 1, 0, r.s, r.l8, r.s, c.batch, c.compute_units).piece_bytes;
+  const size_t gram = plan_of<PARTS>(1, r.s64, r.s64, r.l64, c).piece_bytes;
+  const size_t poly = plan_of<PARTS>(1, r.s64, r.s64, r.s64, c).piece_bytes;
+  const size_t update = plan_of<PARTS>(0, r.s64, r.l64, r.s64, c).piece_bytes;
   size_t pieces = gram > poly ? gram : poly;
   pieces = pieces > update ? pieces : update;
   r.arrivals = take(kArrivalBytes);
@@ -266,76 +290,83 @@ Room carve(const OrthoCall& c) {
   return r;
 }
 
-template <class T, class Op>
+// The operands a b^T of a product: with two parts the segments hi hi, hi lo, lo hi.
+template <int PARTS>
+Problem problem(const Op* a, long a_parts, int lda, const Op* b, long b_parts, int ldb) {
+  Problem p = {};
+  p.a[0] = a;
+  p.b[0] = b;
+  if (PARTS == 2) {
+    p.a[1] = a;
+    p.b[1] = b + b_parts;
+    p.a[2] = a + a_parts;
+    p.b[2] = b;
+  }
+  p.lda = lda;
+  p.ldb = p.ldb1 = ldb;
+  return p;
+}
+
+template <class T, int PARTS>
 int run(const OrthoCall& c) {
-  const Room r = carve<Op>(c);
+  constexpr int SEGS = PARTS == 2 ? 3 : 1;
+  const Room r = carve<PARTS>(c);
   const int tall = c.rows > c.cols;
-  const long x_stride = (long)r.s * r.pitch;
+  const long x_stride = (long)r.s64 * r.pitch;
   Arrivals arrivals = arrivals_at(r.arrivals, true);   // (by norm_kernel)
   const int blocks = c.rows < 4 * NORM_BLOCKS ? (c.rows + 3) / 4 : NORM_BLOCKS;
   PT_TRY(launch(norm_kernel<T>, "orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial, arrivals.set[0], kMaxArrivals));
-  PT_TRY(launch(first_kernel<T, Op>, "orthogonalize: first X", dim3((r.l8 + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
-                r.s, r.l, r.l8, r.pitch, x_stride, r.x[0], (Op*)r.op[0]));
+  PT_TRY(launch(first_kernel<T, PARTS>, "orthogonalize: first X", dim3(r.l64 / 64, r.s64 / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
+                r.s, r.l, r.pitch, x_stride, r.x, r.op[0], r.x_parts));
   const int vec = (uintptr_t)c.o % (4 * sizeof(T)) == 0 && c.ldo % 4 == 0 && c.stride_o % 4 == 0;
-  int cur = 0;
+  const Symmetric<PARTS> A = {r.ao, r.da, r.s64, r.sq, r.sq_parts}, B = {r.bo, r.db, r.s64, r.sq, r.sq_parts};
   for (int k = 0; k < c.steps; ++k) {
-    const float *coefficients = c.coefficients + 3 * k, a = coefficients[0], b = coefficients[1], cc = coefficients[2];
-    const bool last = k + 1 == c.steps && !tall;
-    const Op* x = sizeof(Op) == 2 ? (const Op*)r.op[cur] : (const Op*)r.x[cur];
-    Problem p = {};
-    p.a[0] = p.b[0] = x;
-    p.lda = p.ldb = p.ldb1 = r.pitch;
-    p.M = p.N = r.s;
-    p.M_out = p.N_out = r.s8;
-    p.K = r.l;
+    const Op* x = r.op[k % 2];
+    Problem p = problem<PARTS>(x, r.x_parts, r.pitch, x, r.x_parts, r.pitch);
+    p.M = p.N = p.M_out = p.N_out = r.s64;
+    p.K = r.l64;
     p.batch_a = p.batch_b = x_stride;
-    Symmetric<Op> A = {(Op*)r.ao, r.da, r.s8, r.sq}, B = {(Op*)r.bo, r.db, r.s8, r.sq};
-    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Gram<Op>{A}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: X X^T")));
-    p.a[0] = p.b[0] = r.ao;
-    p.lda = p.ldb = p.ldb1 = r.sq;
-    p.K = r.s;
-    p.batch_a = p.batch_b = (long)r.s8 * r.sq;
-    PT_TRY((run_product<Op, 1, 1, 0, 1, 1>(p, Polynomial<Op>{A, B, b, cc}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: A A")));
-    const int next = 1 - cur;
-    Update<T, Op> u = {};
-    u.from = sizeof(Op) == 2 ? r.x[0] : r.x[cur];
-    u.to = sizeof(Op) == 2 ? r.x[0] : r.x[next];
-    u.op = (Op*)r.op[next];
+    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, Gram<PARTS>{A}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: X X^T")));
+    p = problem<PARTS>(r.ao, r.sq_parts, r.sq, r.ao, r.sq_parts, r.sq);
+    p.M = p.N = p.M_out = p.N_out = p.K = r.s64;
+    p.batch_a = p.batch_b = (long)r.s64 * r.sq;
+    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, Polynomial<PARTS>{A, B, c.coefficients[3 * k + 1], c.coefficients[3 * k + 2]}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: A A")));
+    Update<T, PARTS> u = {};
+    u.x = r.x;
     u.diag = r.db;
+    u.op = r.op[1 - k % 2];
+    u.parts = r.x_parts;
     u.pitch = r.pitch;
     u.diag_pitch = r.sq;
     u.stride = x_stride;
-    u.a = a;
+    u.a = c.coefficients[3 * k];
     u.scale = c.scale;
-    u.out = last ? (T*)c.o : nullptr;
+    u.out = k + 1 == c.steps && !tall ? (T*)c.o : nullptr;
     u.ldo = c.ldo;
+    u.s = r.s;
     u.l = r.l;
     u.vec = vec;
     u.out_stride = c.stride_o;
-    p.a[0] = r.bo;
-    p.b[0] = x;
-    p.ldb = p.ldb1 = r.pitch;
-    p.N = r.l;
-    p.M_out = r.s;
-    p.N_out = r.l8;
+    p = problem<PARTS>(r.bo, r.sq_parts, r.sq, x, r.x_parts, r.pitch);
+    p.M = p.M_out = p.K = r.s64;
+    p.N = p.N_out = r.l64;
+    p.batch_a = (long)r.s64 * r.sq;
     p.batch_b = x_stride;
-    PT_TRY((run_product<Op, 1, 0, 0, 1, 0>(p, u, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: B X")));
-    cur = next;
+    PT_TRY((run_product<Op, 1, 0, 0, SEGS, 0>(p, u, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: B X")));
   }
-  const float* x = sizeof(Op) == 2 ? r.x[0] : r.x[cur];
   if (tall)
-    return launch(transposed_out_kernel<T>, "orthogonalize: output", dim3((r.l + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
+    return launch(transposed_out_kernel<T>, "orthogonalize: output", dim3((r.l + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
   if (c.steps == 0)
-    return launch(out_kernel<T>, "orthogonalize: output", dim3(blocks_for((long)r.s * r.l), 1, c.batch), 256, c.stream, x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
+    return launch(out_kernel<T>, "orthogonalize: output", dim3(blocks_for((long)r.s * r.l), 1, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
   return RL_OK;
 }
 
 }  // namespace
 
-size_t rl_ortho_room(const OrthoCall& c) { return c.dtype == RL_BF16 ? carve<half_t>(c).bytes : carve<float>(c).bytes; }
+size_t rl_ortho_room(const OrthoCall& c) { return c.dtype == RL_BF16 ? carve<1>(c).bytes : carve<2>(c).bytes; }
 
 int rl_ortho_run(const OrthoCall& c) {
-  if (c.dtype == RL_BF16) return run<bf16_t, half_t>(c);
-  if (c.dtype == RL_F16) return run<half_t, float>(c);
-  return run<float, float>(c);
+  if (c.dtype == RL_BF16) return run<bf16_t, 1>(c);
+  if (c.dtype == RL_F16) return run<half_t, 2>(c);
+  return run<float, 2>(c);
 }

@@ -49,9 +49,9 @@ int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream,
   typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, MI, t::BUFS> S;
   static_assert(t::BM == kTiles[K].bm && t::BN == kTiles[K].bn, "the plan's tiles");
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
-  const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits;
+  const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits * batch;
   if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
-  return launch(tile_kernel<S, Epi>, what, dim3((unsigned)groups, 1, batch), S::NT, stream, p, epi);
+  return launch(tile_kernel<S, Epi>, what, dim3((unsigned)groups), S::NT, stream, p, epi);
 }
 
 // Arrival counters of the products of one call, in its workspace: two sets that take turns.  Every product

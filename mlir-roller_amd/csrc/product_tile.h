@@ -284,9 +284,12 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
 
   const int nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const int tiles = S::SYM ? nbm * (nbm + 1) / 2 : nbm * nbn;
-  int pid = blockIdx.x;
-  const int split = pid / tiles;                 // (grid.x = tiles * splits)
-  pid = xcd_order(pid - split * tiles, tiles);
+  // (grid.x = batch * splits * tiles, in this order: a run of it shares operands)
+  int pid = xcd_order(blockIdx.x, gridDim.x);
+  const int batch = pid / (tiles * p.splits);
+  pid -= batch * tiles * p.splits;
+  const int split = pid / tiles;
+  pid -= split * tiles;
   int tile_m, tile_n;
   if constexpr (S::SYM) {
     triangle_tile(pid, nbm, tile_m, tile_n);
@@ -294,10 +297,8 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     panel_tile(pid, nbm, nbn, tile_m, tile_n);
   }
   const int m0 = tile_m * S::BM, n0 = tile_n * S::OUT_N;
-  const int batch = blockIdx.z;
 
-  if (batch == 0)
-    for (int i = blockIdx.x * NT + tid; i < p.n_clear; i += gridDim.x * NT) p.clear[i] = 0;
+  for (int i = blockIdx.x * NT + tid; i < p.n_clear; i += gridDim.x * NT) p.clear[i] = 0;
 
   // K steps of this workgroup.  A segment is a whole number of steps: its last step is cut by K.
   const int seg_steps = (p.K + S::KSTEP - 1) / S::KSTEP;
