@@ -64,7 +64,7 @@ T* pack_space(Carver& room, int rows, int cols, bool need) {
 int pack(FfnMatrix& m, int rows, int cols, T* space, hipStream_t stream) {
   if (!space) return RL_OK;
   const int pitch = pitch_of(cols);
-  PT_TRY(launch(pack_kernel<T>, "packing an operand", dim3(blocks_for((long)rows * (pitch / PER))), 256, stream, (const T*)m.p, m.ld, rows, cols, space, pitch));
+  PT_TRY(launch<pack_kernel<T>>("packing an operand", dim3(blocks_for((long)rows * (pitch / PER))), 256, stream, (const T*)m.p, m.ld, rows, cols, space, pitch));
   m = {space, pitch};
   return RL_OK;
 }
@@ -102,6 +102,7 @@ struct ForwardRoom {
   T *x, *w_gate, *w_up, *w_down, *h;
   float* h32;
   char *arrivals, *pieces;
+  Plan up, down;
   bool few;   // takes few_rows_kernel
   size_t bytes;
 };
@@ -124,9 +125,9 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
     r.w_up = pack_space(room, c.F, c.D, pack && (unaligned || !aligned(c.w_up)));
     r.w_down = pack_space(room, c.D, c.F, pack && (unaligned || !aligned(c.w_down)));
     r.arrivals = room.take(kArrivalBytes);
-    const size_t up = plan_product(ES, 1, 1, 0, c.T, c.F, c.D, 1, c.compute_units, 0, kFewRowsTile + 1).piece_bytes;
-    const size_t down = plan_product(ES, 0, 1, 0, c.T, c.D, c.F, 1, c.compute_units, 0, kFewRowsTile + 1).piece_bytes;
-    r.pieces = room.take(larger(up, down));
+    r.up = plan_for<T, 1, 1, 1, 1, 0>(c.T, c.F, c.D, 1, c.compute_units);
+    r.down = plan_for<T, 1, 1, 0, 1, 0>(c.T, c.D, c.F, 1, c.compute_units);
+    r.pieces = room.take(larger(r.up.piece_bytes, r.down.piece_bytes));
   }
   r.bytes = room.used();
   return r;
@@ -144,9 +145,9 @@ int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated
   constexpr int ROWS = 16 / PARTS;
   typedef typename x_type<T, SPLIT>::type H;
   const int up = (c.F + ROWS - 1) / ROWS, down = (c.D + ROWS - 1) / ROWS;
-  PT_TRY(launch(few_rows_kernel<T, BLOCKS, PARTS, 1, 0, GatedForward<T, KIND>>, "ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
+  PT_TRY(launch<few_rows_kernel<T, BLOCKS, PARTS, 1, 0, GatedForward<T, KIND>>>("ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
                 (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, c.D, gated));
-  return launch(few_rows_kernel<T, BLOCKS, PARTS, 0, SPLIT, Store<T>>, "ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
+  return launch<few_rows_kernel<T, BLOCKS, PARTS, 0, SPLIT, Store<T>>>("ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
                 c.D, c.F, out);
 }
 
@@ -182,9 +183,9 @@ int forward_as(const FfnCall& call) {
   Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, c.F);
   up.b[1] = c.w_up.p;
   up.ldb1 = c.w_up.ld;
-  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: gate and up")));
+  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, r.up, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: gate and up")));
   const Problem down = problem(gated.h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
-  return run_product<T, 1, 1, 0, 1, 0>(down, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: down");
+  return run_product<T, 1, 1, 0, 1, 0>(down, r.down, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: down");
 }
 
 int forward(const FfnCall& c) {
@@ -196,6 +197,7 @@ int forward(const FfnCall& c) {
 struct BackwardRoom {
   T *dy, *x, *w_gate, *w_up, *w_down, *dg, *du;
   char *arrivals, *pieces;
+  Plan dw_down, dh, dx, dw;   // (dw: gate and up)
   size_t bytes;
 };
 
@@ -215,10 +217,11 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
   r.w_up = pack_space(room, c.F, c.D, weights);
   r.w_down = pack_space(room, c.D, c.F, unaligned || !aligned(c.w_down));
   r.arrivals = room.take(kArrivalBytes);
-  size_t pieces = plan_product(ES, 0, 1, 0, c.T, c.F, c.D, 1, c.compute_units).piece_bytes;
-  pieces = larger(pieces, plan_product(ES, 0, 2, 0, c.T, c.D, c.F, 1, c.compute_units).piece_bytes);
-  pieces = larger(pieces, plan_product(ES, 0, 1, 0, c.F, c.D, c.T, 2, c.compute_units).piece_bytes);
-  pieces = larger(pieces, plan_product(ES, 0, 1, 0, c.D, c.F, c.T, 1, c.compute_units).piece_bytes);
+  r.dw_down = plan_for<T, 0, 0, 0, 1, 0>(c.D, c.F, c.T, 1, c.compute_units);
+  r.dh = plan_for<T, 1, 0, 0, 1, 0>(c.T, c.F, c.D, 1, c.compute_units);
+  r.dx = plan_for<T, 1, 0, 0, 2, 0>(c.T, c.D, c.F, 1, c.compute_units);
+  r.dw = plan_for<T, 0, 0, 0, 1, 0>(c.F, c.D, c.T, 2, c.compute_units);
+  const size_t pieces = larger(larger(r.dw_down.piece_bytes, r.dh.piece_bytes), larger(r.dx.piece_bytes, r.dw.piece_bytes));
   r.pieces = room.take(pieces);
   r.bytes = room.used();
   return r;
@@ -227,7 +230,7 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
 size_t backward_room(const FfnCall& c, bool unaligned) { return backward_carve(c, unaligned).bytes; }
 
 int zero(void* p, int ld, int rows, int cols, hipStream_t stream) {
-  return launch(zero_kernel<T>, "ffn: zero gradient", dim3(blocks_for((long)rows * cols)), 256, stream, (T*)p, ld, rows, cols);
+  return launch<zero_kernel<T>>("ffn: zero gradient", dim3(blocks_for((long)rows * cols)), 256, stream, (T*)p, ld, rows, cols);
 }
 
 template <int KIND>
@@ -238,7 +241,7 @@ int gated_backward(const FfnCall& c, const BackwardRoom& r, const FfnSaved& s, c
   gated.dg = r.dg;
   gated.du = r.du;
   gated.pitch = s.pitch;
-  return run_product<T, 1, 0, 0, 1, 0>(dh, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dh");
+  return run_product<T, 1, 0, 0, 1, 0>(dh, r.dh, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dh");
 }
 
 int backward(const FfnCall& call) {
@@ -256,7 +259,7 @@ int backward(const FfnCall& call) {
   PT_TRY(pack(c.dy, c.T, c.D, r.dy, c.stream));
   if (c.dw_down) {
     const Problem p = problem(c.dy.p, c.dy.ld, h, s.pitch, c.D, c.F, c.T, c.D, c.F);
-    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, store(c.dw_down, c.ld_dw_down, c.F), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_down")));
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, r.dw_down, store(c.dw_down, c.ld_dw_down, c.F), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_down")));
   }
   if (!c.dx && !c.dw_gate) return RL_OK;
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
@@ -272,7 +275,7 @@ int backward(const FfnCall& call) {
     Problem p = problem(r.dg, s.pitch, c.w_gate.p, c.w_gate.ld, c.T, c.D, c.F, c.T, c.D);
     p.a[1] = r.du;
     p.b[1] = c.w_up.p;
-    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, store(c.dx, c.ld_dx, c.D), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
+    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, r.dx, store(c.dx, c.ld_dx, c.D), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
   }
   if (c.dw_gate) {
     PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
@@ -282,7 +285,7 @@ int backward(const FfnCall& call) {
     out.c[1] = (T*)c.dw_up;
     out.ldc1 = c.ld_dw_up;
     out.vec = out.vec && vec_ok(c.dw_up, c.ld_dw_up);
-    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, out, 2, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
+    PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, r.dw, out, 2, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
   }
   return RL_OK;
 }

@@ -239,6 +239,7 @@ struct Room {
   float *da, *db;
   double* partial;
   char *arrivals, *pieces;
+  Plan gram, poly, update;
   int s, l;        // sides of X
   int l64, s64;    // the same up to whole K steps: rows and columns that exist, zeros beyond s and l
   int pitch, sq;   // elements from row to row of X, and of A and B
@@ -247,11 +248,6 @@ struct Room {
 };
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
-template <int PARTS>
-Plan plan_of(int sym, int M_out, int N_out, int K, const OrthoCall& c) {
-  return plan_product(sizeof(Op), 0, PARTS == 2 ? 3 : 1, sym, M_out, N_out, K, c.batch, c.compute_units, 0, sym || PARTS == 2 ? kFewRowsTile : tiles_end<1, 0, 1, 0>());
-}
 
 template <int PARTS>
 Room carve(const OrthoCall& c) {
@@ -279,11 +275,12 @@ Room carve(const OrthoCall& c) {
   r.da = (float*)take((size_t)c.batch * r.sq * 4);
   r.db = (float*)take((size_t)c.batch * r.sq * 4);
   r.partial = (double*)take((size_t)c.batch * NORM_BLOCKS * 8);
-  const size_t gram = plan_of<PARTS>(1, r.s64, r.s64, r.l64, c).piece_bytes;
-  const size_t poly = plan_of<PARTS>(1, r.s64, r.s64, r.s64, c).piece_bytes;
-  const size_t update = plan_of<PARTS>(0, r.s64, r.l64, r.s64, c).piece_bytes;
-  size_t pieces = gram > poly ? gram : poly;
-  pieces = pieces > update ? pieces : update;
+  constexpr int SEGS = PARTS == 2 ? 3 : 1;
+  r.gram = plan_for<Op, 1, 1, 0, SEGS, 1>(r.s64, r.s64, r.l64, c.batch, c.compute_units);
+  r.poly = plan_for<Op, 1, 1, 0, SEGS, 1>(r.s64, r.s64, r.s64, c.batch, c.compute_units);
+  r.update = plan_for<Op, 1, 0, 0, SEGS, 0>(r.s64, r.l64, r.s64, c.batch, c.compute_units);
+  size_t pieces = r.gram.piece_bytes > r.poly.piece_bytes ? r.gram.piece_bytes : r.poly.piece_bytes;
+  pieces = pieces > r.update.piece_bytes ? pieces : r.update.piece_bytes;
   r.arrivals = take(kArrivalBytes);
   r.pieces = take(pieces);
   r.bytes = used;
@@ -315,8 +312,8 @@ int run(const OrthoCall& c) {
   const long x_stride = (long)r.s64 * r.pitch;
   Arrivals arrivals = arrivals_at(r.arrivals, true);   // (by norm_kernel)
   const int blocks = c.rows < 4 * NORM_BLOCKS ? (c.rows + 3) / 4 : NORM_BLOCKS;
-  PT_TRY(launch(norm_kernel<T>, "orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial, arrivals.set[0], kMaxArrivals));
-  PT_TRY(launch(first_kernel<T, PARTS>, "orthogonalize: first X", dim3(r.l64 / 64, r.s64 / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
+  PT_TRY(launch<norm_kernel<T>>("orthogonalize: norm", dim3(blocks, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, c.rows, c.cols, r.partial, arrivals.set[0], kMaxArrivals));
+  PT_TRY(launch<first_kernel<T, PARTS>>("orthogonalize: first X", dim3(r.l64 / 64, r.s64 / 64, c.batch), 256, c.stream, (const T*)c.g, c.ldg, c.stride_g, tall, (const double*)r.partial, blocks, c.eps,
                 r.s, r.l, r.pitch, x_stride, r.x, r.op[0], r.x_parts));
   const int vec = (uintptr_t)c.o % (4 * sizeof(T)) == 0 && c.ldo % 4 == 0 && c.stride_o % 4 == 0;
   const Symmetric<PARTS> A = {r.ao, r.da, r.s64, r.sq, r.sq_parts}, B = {r.bo, r.db, r.s64, r.sq, r.sq_parts};
@@ -326,11 +323,11 @@ int run(const OrthoCall& c) {
     p.M = p.N = p.M_out = p.N_out = r.s64;
     p.K = r.l64;
     p.batch_a = p.batch_b = x_stride;
-    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, Gram<PARTS>{A}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: X X^T")));
+    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, r.gram, Gram<PARTS>{A}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: X X^T")));
     p = problem<PARTS>(r.ao, r.sq_parts, r.sq, r.ao, r.sq_parts, r.sq);
     p.M = p.N = p.M_out = p.N_out = p.K = r.s64;
     p.batch_a = p.batch_b = (long)r.s64 * r.sq;
-    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, Polynomial<PARTS>{A, B, c.coefficients[3 * k + 1], c.coefficients[3 * k + 2]}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: A A")));
+    PT_TRY((run_product<Op, 1, 1, 0, SEGS, 1>(p, r.poly, Polynomial<PARTS>{A, B, c.coefficients[3 * k + 1], c.coefficients[3 * k + 2]}, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: A A")));
     Update<T, PARTS> u = {};
     u.x = r.x;
     u.diag = r.db;
@@ -352,12 +349,12 @@ int run(const OrthoCall& c) {
     p.N = p.N_out = r.l64;
     p.batch_a = (long)r.s64 * r.sq;
     p.batch_b = x_stride;
-    PT_TRY((run_product<Op, 1, 0, 0, SEGS, 0>(p, u, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: B X")));
+    PT_TRY((run_product<Op, 1, 0, 0, SEGS, 0>(p, r.update, u, c.batch, r.pieces, arrivals, c.stream, c.compute_units, "orthogonalize: B X")));
   }
   if (tall)
-    return launch(transposed_out_kernel<T>, "orthogonalize: output", dim3((r.l + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
+    return launch<transposed_out_kernel<T>>("orthogonalize: output", dim3((r.l + 63) / 64, (r.s + 63) / 64, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
   if (c.steps == 0)
-    return launch(out_kernel<T>, "orthogonalize: output", dim3(blocks_for((long)r.s * r.l), 1, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
+    return launch<out_kernel<T>>("orthogonalize: output", dim3(blocks_for((long)r.s * r.l), 1, c.batch), 256, c.stream, (const float*)r.x, r.s, r.l, r.pitch, x_stride, c.scale, (T*)c.o, c.ldo, c.stride_o);
   return RL_OK;
 }
 

@@ -3,27 +3,43 @@
 #ifndef PRODUCT_LAUNCH_H
 #define PRODUCT_LAUNCH_H
 
+#include <atomic>
+
 #include "product_ops.h"
 #include "product_plan.h"
 #include "roller_hip.h"
 #include "roller_internal.h"
 
-#define PT_TRY(expr)              \
+#define PT_TRY(...)               \
   do {                            \
-    const int rc_ = (expr);       \
+    const int rc_ = (__VA_ARGS__); \
     if (rc_) return rc_;          \
   } while (0)
 
 namespace product {
 
+// (the arguments converted to the kernel's parameter types, then their addresses)
 template <class... Params, class... Args>
-int launch(void (*kernel)(Params...), const char* what, dim3 grid, int threads, hipStream_t stream, Args... args) {
-  // (the arguments converted to the kernel's parameter types, then their addresses)
+int launch_function(hipFunction_t f, void (*)(Params...), const char* what, dim3 grid, int threads, hipStream_t stream, Args... args) {
   return [&](Params... p) {
     void* ptrs[] = {(void*)&p...};
-    const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), ptrs, 0, stream);
+    const hipError_t e = hipModuleLaunchKernel(f, grid.x, grid.y, grid.z, threads, 1, 1, 0, stream, ptrs, nullptr);
     return e == hipSuccess ? RL_OK : rl_hip_fail(e, what);
   }(args...);
+}
+
+// Launches KERNEL.  Its function is looked up once: a launch by symbol looks it up every time, which a call of
+// two short kernels notices.
+template <auto KERNEL, class... Args>
+int launch(const char* what, dim3 grid, int threads, hipStream_t stream, Args... args) {
+  static std::atomic<hipFunction_t> known{nullptr};
+  hipFunction_t f = known.load(std::memory_order_relaxed);
+  if (!f) {
+    const hipError_t e = hipGetFuncBySymbol(&f, (const void*)KERNEL);
+    if (e != hipSuccess) return rl_hip_fail(e, what);
+    known.store(f, std::memory_order_relaxed);
+  }
+  return launch_function(f, KERNEL, what, grid, threads, stream, args...);
 }
 
 inline unsigned blocks_for(long items) {
@@ -51,7 +67,7 @@ int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream,
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits * batch;
   if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
-  return launch(tile_kernel<S, Epi>, what, dim3((unsigned)groups), S::NT, stream, p, epi);
+  return launch<tile_kernel<S, Epi>>(what, dim3((unsigned)groups), S::NT, stream, p, epi);
 }
 
 // Arrival counters of the products of one call, in its workspace: two sets that take turns.  Every product
@@ -80,19 +96,23 @@ inline int take_plan(Problem& p, const Plan& plan, void* room, Arrivals& arrival
   p.clear = arrivals.set[arrivals.turn];
   p.n_clear = kMaxArrivals;
   if (p.splits > 1 && !arrivals.ready)
-    PT_TRY(launch(zero_kernel<unsigned>, "clearing arrival counters", dim3(kMaxArrivals / 256), 256, stream, p.arrivals, kMaxArrivals, 1, kMaxArrivals));
+    PT_TRY(launch<zero_kernel<unsigned>>("clearing arrival counters", dim3(kMaxArrivals / 256), 256, stream, p.arrivals, kMaxArrivals, 1, kMaxArrivals));
   arrivals.ready = true;
   return RL_OK;
 }
 
-// The product `p` (extents, operands) with epilogue `epi`: tile and split by plan_product, pieces of split
-// tiles in `room` (piece_bytes of the plan).
+// The plan of a product of these forms.
+template <class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM>
+Plan plan_for(int M_out, int N_out, int K, int batch, int compute_units, int max_splits = kMaxSplits) {
+  return plan_product(sizeof(T), GATED, SEGS, SYM, M_out, N_out, K, batch, compute_units, tiles_end<A_KM, B_KM, SEGS, SYM>(), max_splits);
+}
+
+// The product `p` (extents, operands) with epilogue `epi` by `plan`; pieces of split tiles in `room`
+// (piece_bytes of the plan).
 template <class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
-int run_product(Problem p, const Epi& epi, int batch, void* room, Arrivals& arrivals, hipStream_t stream, int compute_units, const char* what) {
-  constexpr int END = tiles_end<A_KM, B_KM, SEGS, SYM>();
-  Plan plan = plan_product(sizeof(T), GATED, SEGS, SYM, p.M_out, p.N_out, p.K, batch, compute_units, 0, END);
+int run_product(Problem p, Plan plan, const Epi& epi, int batch, void* room, Arrivals& arrivals, hipStream_t stream, int compute_units, const char* what) {
   if (plan.splits > 1 && !arrivals.ready) {
-    const Plan whole = plan_product(sizeof(T), GATED, SEGS, SYM, p.M_out, p.N_out, p.K, batch, compute_units, 0, END, 1);
+    const Plan whole = plan_for<T, A_KM, B_KM, GATED, SEGS, SYM>(p.M_out, p.N_out, p.K, batch, compute_units, 1);
     if (whole.time < plan.time + kClearLaunch) plan = whole;
   }
   PT_TRY(take_plan(p, plan, room, arrivals, stream));
@@ -103,7 +123,7 @@ int run_product(Problem p, const Epi& epi, int batch, void* room, Arrivals& arri
     case 3: return launch_tile<3, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
     default: break;
   }
-  if constexpr (END > kFewRowsTile) return launch_tile<kFewRowsTile, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
+  if constexpr (tiles_end<A_KM, B_KM, SEGS, SYM>() > kFewRowsTile) return launch_tile<kFewRowsTile, T, A_KM, B_KM, GATED, SEGS, SYM>(p, epi, batch, stream, what);
   else return RL_OK;
 }
 

@@ -41,11 +41,11 @@ struct Plan {
   size_t piece_bytes;
 };
 
-inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out, int N_out, int K, int batch, int compute_units, int first_tile = 0, int tiles_end = kFewRowsTile, int max_splits = kMaxSplits) {
+inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out, int N_out, int K, int batch, int compute_units, int tiles_end, int max_splits = kMaxSplits) {
   Plan best = {};
   const int kstep = 128 / elem_bytes;
   const int steps = (K + kstep - 1) / kstep * segs;
-  for (int t = first_tile; t < tiles_end; ++t) {
+  for (int t = 0; t < tiles_end; ++t) {
     const TileCost& c = kTiles[t];
     const int out_n = gated ? c.bn / 2 : c.bn;
     const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + out_n - 1) / out_n;

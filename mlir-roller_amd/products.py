@@ -18,7 +18,7 @@ import ctypes as C
 from typing import Optional, Sequence
 
 from . import hip
-from .hip import FfnConfig, OrthoConfig, _address, _stream_handle, check, lib
+from .hip import FfnConfig, OrthoConfig, Ptr, _stream_handle, check, lib
 
 DTYPES = {"fp32": 0, "fp16": 1, "bf16": 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
@@ -28,6 +28,11 @@ def _choice(what: str, value: str, table: dict) -> int:
     if value not in table:
         raise ValueError(f"{what} is one of {', '.join(table)}, got {value!r}")
     return table[value]
+
+
+def _address(x) -> int:
+    """``hip._address``, for a call that takes a handful of them and may last a few microseconds."""
+    return x.address if type(x) is Ptr else hip._address(x)
 
 
 def _room(workspace, workspace_bytes: Optional[int]) -> tuple[Optional[int], int]:
