@@ -321,6 +321,17 @@ int rl_ffn_backward(const rl_ffn_config* cfg, const void* dy, int lddy, const vo
                     int lddx, void* dw_gate, int ldd_gate, void* dw_up, int ldd_up, void* dw_down, int ldd_down, int T,
                     void* workspace, size_t workspace_bytes, rl_stream stream);
 
+/* The tile of a matrix product and the number of workgroups that share the K steps of each. */
+typedef struct rl_product_tile {
+  int rows, cols; /* of the product (gate and up columns count both) */
+  int splits;
+} rl_product_tile;
+
+/* What the products of a block of T tokens run with on a device of `compute_units` CUs (host arithmetic, no
+ * device needed): gate and up, down; backward: dw_down, dh, dx, dw_gate with dw_up.  Counterpart of
+ * rl_gemm_streamk_schedule above; up to 16 tokens forward take no tiles. */
+int rl_ffn_tiles(const rl_ffn_config* cfg, int T, int compute_units, rl_product_tile out[6]);
+
 /* Orthogonalises a matrix, or each of a stack of `batch`, by Newton-Schulz products (the update of the Muon
  * optimiser): X = G / (||G||_F + eps); steps times X <- a X + (b A + c A A) X with A = X X^T (of the
  * shorter side); O = scale * X.  G[rows, cols] and O[rows, cols] are of type dtype; O may be G. */
@@ -332,6 +343,9 @@ typedef struct rl_ortho_config {
 } rl_ortho_config;
 
 int rl_ortho_workspace_bytes(const rl_ortho_config* cfg, size_t* bytes);
+
+/* The same for the products X X^T, A A and B X of a step. */
+int rl_ortho_tiles(const rl_ortho_config* cfg, int compute_units, rl_product_tile out[3]);
 
 /* `coefficients`: host memory, (a, b, c) for each step, read before the call returns; NULL: 3.4445, -4.7750,
  * 2.0315 in every step.  They must keep |X| and |A| below 100 (operands are fp16 inside; any

@@ -96,6 +96,22 @@ Problem problem(const void* a, int lda, const void* b, int ldb, int M, int N, in
 
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
+Plan plan_up(const FfnCall& c) { return plan_for<T, 1, 1, 1, 1, 0>(c.T, c.F, c.D, 1, c.compute_units); }
+Plan plan_down(const FfnCall& c) { return plan_for<T, 1, 1, 0, 1, 0>(c.T, c.D, c.F, 1, c.compute_units); }
+Plan plan_dw_down(const FfnCall& c) { return plan_for<T, 0, 0, 0, 1, 0>(c.D, c.F, c.T, 1, c.compute_units); }
+Plan plan_dh(const FfnCall& c) { return plan_for<T, 1, 0, 0, 1, 0>(c.T, c.F, c.D, 1, c.compute_units); }
+Plan plan_dx(const FfnCall& c) { return plan_for<T, 1, 0, 0, 2, 0>(c.T, c.D, c.F, 1, c.compute_units); }
+Plan plan_dw(const FfnCall& c) { return plan_for<T, 0, 0, 0, 1, 0>(c.F, c.D, c.T, 2, c.compute_units); }
+
+void plans(const FfnCall& c, Plan out[6]) {
+  out[0] = plan_up(c);
+  out[1] = plan_down(c);
+  out[2] = plan_dw_down(c);
+  out[3] = plan_dh(c);
+  out[4] = plan_dx(c);
+  out[5] = plan_dw(c);
+}
+
 // ---- forward ----
 
 struct ForwardRoom {
@@ -125,8 +141,8 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
     r.w_up = pack_space(room, c.F, c.D, pack && (unaligned || !aligned(c.w_up)));
     r.w_down = pack_space(room, c.D, c.F, pack && (unaligned || !aligned(c.w_down)));
     r.arrivals = room.take(kArrivalBytes);
-    r.up = plan_for<T, 1, 1, 1, 1, 0>(c.T, c.F, c.D, 1, c.compute_units);
-    r.down = plan_for<T, 1, 1, 0, 1, 0>(c.T, c.D, c.F, 1, c.compute_units);
+    r.up = plan_up(c);
+    r.down = plan_down(c);
     r.pieces = room.take(larger(r.up.piece_bytes, r.down.piece_bytes));
   }
   r.bytes = room.used();
@@ -217,10 +233,10 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
   r.w_up = pack_space(room, c.F, c.D, weights);
   r.w_down = pack_space(room, c.D, c.F, unaligned || !aligned(c.w_down));
   r.arrivals = room.take(kArrivalBytes);
-  r.dw_down = plan_for<T, 0, 0, 0, 1, 0>(c.D, c.F, c.T, 1, c.compute_units);
-  r.dh = plan_for<T, 1, 0, 0, 1, 0>(c.T, c.F, c.D, 1, c.compute_units);
-  r.dx = plan_for<T, 1, 0, 0, 2, 0>(c.T, c.D, c.F, 1, c.compute_units);
-  r.dw = plan_for<T, 0, 0, 0, 1, 0>(c.F, c.D, c.T, 2, c.compute_units);
+  r.dw_down = plan_dw_down(c);
+  r.dh = plan_dh(c);
+  r.dx = plan_dx(c);
+  r.dw = plan_dw(c);
   const size_t pieces = larger(larger(r.dw_down.piece_bytes, r.dh.piece_bytes), larger(r.dx.piece_bytes, r.dw.piece_bytes));
   r.pieces = room.take(pieces);
   r.bytes = room.used();
@@ -292,4 +308,4 @@ int backward(const FfnCall& call) {
 
 }  // namespace
 
-FfnType FFN_TABLE() { return {forward_room, backward_room, forward, backward}; }
+FfnType FFN_TABLE() { return {plans, forward_room, backward_room, forward, backward}; }

@@ -367,3 +367,10 @@ int rl_ortho_run(const OrthoCall& c) {
   if (c.dtype == RL_F16) return run<half_t, 2>(c);
   return run<float, 2>(c);
 }
+
+void rl_ortho_plans(const OrthoCall& c, Plan out[3]) {
+  const Room r = c.dtype == RL_BF16 ? carve<1>(c) : carve<2>(c);
+  out[0] = r.gram;
+  out[1] = r.poly;
+  out[2] = r.update;
+}

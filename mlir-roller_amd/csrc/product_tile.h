@@ -116,17 +116,18 @@ struct mma {
 // Permutation of the 16-byte chunks of row k of a row-major tile whose rows are ROW_BYTES long (XOR-ed
 // onto the chunk number).
 //   16 bits: half a wave reads 64 bytes (32 rows of the product) from each of the rows k .. k+3; the four
-//   must lie in four different quarters of the 256 bytes that the banks span.  A row of 128 bytes already
-//   differs from its neighbour by its own length.
+//   must lie in four different quarters of the 256 bytes that the banks span.  Where a row is an odd multiple
+//   of 128 bytes (tiles of 64 and 192), every second row differs from its neighbour by its own length already;
+//   and its number of chunks allows no permutation beyond groups of eight.
 //   32 bits: half a wave reads 128 bytes of one row, which covers the 32 banks of a 32-bit read as it is.
 template <int ES, int ROW_BYTES>
 PT_DEV constexpr int mn_swizzle(int k) {
+  static_assert(ROW_BYTES % 128 == 0, "tiles are multiples of 64 rows of 16 bits");
   if constexpr (ES == 4) {
     return 0;
-  } else if constexpr (ROW_BYTES >= 256) {
+  } else if constexpr (ROW_BYTES % 256 == 0) {
     return (k & 3) * 4;
   } else {
-    static_assert(ROW_BYTES == 128, "tiles are at least 64 rows of 16 bits");
     return ((k >> 1) & 1) * 4;
   }
 }

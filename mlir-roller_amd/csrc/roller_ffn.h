@@ -46,6 +46,7 @@ inline FfnSaved ffn_saved(int es, int T, int F) {
 // One set of functions per element type.  `room` sizes count packed copies only where the call needs them:
 // the matrices of `c` decide (pointers and leading dimensions; for a size question with `unaligned`, all).
 struct FfnType {
+  void (*plans)(const FfnCall& c, product::Plan out[6]);   // gate and up, down, dw_down, dh, dx, dw_gate and dw_up
   size_t (*forward_room)(const FfnCall& c, bool unaligned);
   size_t (*backward_room)(const FfnCall& c, bool unaligned);
   int (*forward)(const FfnCall& c);

@@ -7,6 +7,8 @@
 
 #include <cstddef>
 
+#include "product_plan.h"
+
 struct OrthoCall {
   int dtype, rows, cols, batch, steps;
   const float* coefficients;   // steps x (a, b, c), host memory
@@ -21,6 +23,7 @@ struct OrthoCall {
 };
 
 __attribute__((visibility("hidden"))) size_t rl_ortho_room(const OrthoCall& c);
+__attribute__((visibility("hidden"))) void rl_ortho_plans(const OrthoCall& c, product::Plan out[3]);
 __attribute__((visibility("hidden"))) int rl_ortho_run(const OrthoCall& c);
 
 #endif

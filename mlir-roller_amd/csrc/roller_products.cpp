@@ -74,6 +74,8 @@ int check_tokens(int T) {
 
 FfnType type_of(int dtype) { return dtype == RL_F32 ? rl_ffn_f32() : dtype == RL_F16 ? rl_ffn_f16() : rl_ffn_bf16(); }
 
+rl_product_tile tile_of(const product::Plan& p) { return {product::kTiles[p.tile].bm, product::kTiles[p.tile].bn, p.splits}; }
+
 #define TRY(expr)          \
   do {                     \
     const int rc_ = (expr); \
@@ -178,6 +180,23 @@ int rl_ffn_workspace_bytes(const rl_ffn_config* cfg, int T, int backward, int un
       if (b > need) need = b;
     }
     *bytes = need;
+    return RL_OK;
+  });
+}
+
+int rl_ffn_tiles(const rl_ffn_config* cfg, int T, int compute_units, rl_product_tile out[6]) {
+  return guarded([&]() -> int {
+    TRY(check_ffn(cfg));
+    TRY(check_tokens(T));
+    if (!out || T == 0 || compute_units < 1) return rl_fail(RL_ERR_INVALID_ARG, "rl_ffn_tiles: needs tokens, compute units and a place to write to");
+    FfnCall c = {};
+    c.T = T;
+    c.D = cfg->d_model;
+    c.F = cfg->d_ff;
+    c.compute_units = compute_units;
+    product::Plan plans[6];
+    type_of(cfg->dtype).plans(c, plans);
+    for (int i = 0; i < 6; ++i) out[i] = tile_of(plans[i]);
     return RL_OK;
   });
 }
@@ -288,6 +307,23 @@ int rl_ortho_workspace_bytes(const rl_ortho_config* cfg, size_t* bytes) {
     c.batch = cfg->batch;
     c.steps = cfg->steps;
     *bytes = rl_ortho_room(c);
+    return RL_OK;
+  });
+}
+
+int rl_ortho_tiles(const rl_ortho_config* cfg, int compute_units, rl_product_tile out[3]) {
+  return guarded([&]() -> int {
+    TRY(check_ortho(cfg));
+    if (!out || cfg->batch == 0 || compute_units < 1) return rl_fail(RL_ERR_INVALID_ARG, "rl_ortho_tiles: needs matrices, compute units and a place to write to");
+    OrthoCall c = {};
+    c.dtype = cfg->dtype;
+    c.rows = cfg->rows;
+    c.cols = cfg->cols;
+    c.batch = cfg->batch;
+    c.compute_units = compute_units;
+    product::Plan plans[3];
+    rl_ortho_plans(c, plans);
+    for (int i = 0; i < 3; ++i) out[i] = tile_of(plans[i]);
     return RL_OK;
   });
 }

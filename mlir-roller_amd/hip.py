@@ -76,6 +76,11 @@ class OrthoConfig(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dtype", "rows", "cols", "batch", "steps")] + [("eps", C.c_float), ("scale", C.c_float)]
 
 
+class ProductTile(C.Structure):
+    """``rl_product_tile``: the tile of a matrix product and its split."""
+    _fields_ = [(n, C.c_int) for n in ("rows", "cols", "splits")]
+
+
 class StreamKSchedule(C.Structure):
     """``rl_streamk_schedule``: how a stream-K configuration splits one problem."""
     _fields_ = [("grid", C.c_int), ("k_steps", C.c_int), ("tiles", C.c_int), ("tile_rows", C.c_int), ("tile_cols", C.c_int),
@@ -227,6 +232,8 @@ _SIGNATURES = {
     "rl_gemm_streamk_segments": ([C.POINTER(_GemmConfigC)] + [C.c_int] * 5 + [C.POINTER(StreamKSegment), C.c_int, C.POINTER(C.c_int)], C.c_int),
     "rl_ffn_workspace_bytes": ([C.POINTER(FfnConfig), C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "rl_ffn_saved_bytes": ([C.POINTER(FfnConfig), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "rl_ffn_tiles": ([C.POINTER(FfnConfig), C.c_int, C.c_int, C.POINTER(ProductTile)], C.c_int),
+    "rl_ortho_tiles": ([C.POINTER(OrthoConfig), C.c_int, C.POINTER(ProductTile)], C.c_int),
     "rl_ffn_forward": ([C.POINTER(FfnConfig)] + [C.c_void_p, C.c_int] * 5 + [C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),
     "rl_ffn_backward": ([C.POINTER(FfnConfig)] + [C.c_void_p, C.c_int] * 5 + [C.c_void_p] + [C.c_void_p, C.c_int] * 4
                         + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p], C.c_int),

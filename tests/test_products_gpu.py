@@ -134,6 +134,24 @@ def test_forward_and_backward(device, T, D, F, dtype, act):
     assert np.array_equal(kept, saved.get())                    # the backward pass only reads it
 
 
+# Sizes that between them take every product through every tile, whole and split (test_products.py counts).
+EVERY_TILE = [(34, 66, 79, "bf16"), (625, 1732, 3374, "fp16"), (33, 568, 3752, "bf16"), (2162, 72, 110, "fp16"), (257, 1802, 64, "bf16"), (1325, 1546, 80, "fp16"),
+              (2140, 67, 2055, "bf16"), (2421, 2066, 85, "fp16"), (35, 323, 2866, "bf16"), (386, 65, 2729, "bf16"), (1174, 71, 3259, "fp16"), (96, 2398, 3940, "bf16"),
+              (2422, 106, 3708, "bf16"), (1023, 1920, 1000, "fp16"), (1000, 640, 3000, "bf16"),
+              (46, 69, 64, "fp32"), (32, 1710, 1660, "fp32"), (1963, 72, 1583, "fp32"), (2412, 1372, 68, "fp32"), (38, 1586, 4035, "fp32"), (2186, 81, 3130, "fp32"),
+              (67, 70, 2774, "fp32"), (2451, 214, 66, "fp32"), (37, 324, 3112, "fp32"), (443, 64, 2813, "fp32")]
+
+
+@pytest.mark.parametrize("T,D,F,dtype", EVERY_TILE)
+def test_every_tile(device, T, D, F, dtype):
+    b = Block(T, D, F, dtype, "silu")
+    saved = room(b.op.saved_bytes(T))
+    b.forward(saved)
+    b.check_y()
+    b.backward(saved)
+    b.check_grads()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("T", [5, 40, 150])
 @pytest.mark.parametrize("pad,shift,pad_up", [(8, 0, 24), (3, 1, 3), (0, 5, 0), (16, 8, 9)])
