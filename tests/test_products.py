@@ -126,3 +126,31 @@ def test_dtypes_and_activations_match_the_header():
     assert products.DTYPES == {"fp32": value("RL_F32"), "fp16": value("RL_F16"), "bf16": value("RL_BF16")}
     assert products.ACTIVATIONS == {"silu": value("RL_ACT_SILU"), "gelu": value("RL_ACT_GELU"), "gelu_tanh": value("RL_ACT_GELU_TANH")}
     assert Ptr(256).address == 256
+
+
+def kinds(tiles):
+    """(product, tile rows, split or not) of every product in the result of tiles()."""
+    return {(name, rows, splits > 1) for name, (rows, _, splits) in tiles.items()}
+
+
+def test_the_sizes_of_the_gpu_tests_take_every_product_through_every_tile(hip_lib):
+    import random
+    from test_products_gpu import EVERY_ORTHO_TILE, EVERY_TILE, EVERY_TILE_SAMPLED
+    pick = random.Random(1)
+    between = lambda lo, hi: int(2 ** pick.uniform(lo, hi))
+    for dtypes in (("bf16", "fp16"), ("fp32",)):
+        reached = set().union(*(kinds(GatedFfn(between(6, 14), between(6, 14), dtypes[0]).tiles(between(5, 14))) for _ in range(4000)))
+        tested = set().union(*(kinds(GatedFfn(D, F, dtype).tiles(T)) for T, D, F, dtype in EVERY_TILE + EVERY_TILE_SAMPLED if dtype in dtypes))
+        assert len(reached) > 25 and reached <= tested, reached - tested
+    for dtypes in (("bf16",), ("fp16", "fp32")):
+        reached = set().union(*(kinds(Orthogonalizer(between(5, 13), between(5, 13), between(0, 6), dtypes[0]).tiles()) for _ in range(4000)))
+        tested = set().union(*(kinds(Orthogonalizer(m, n, batch, dtype).tiles()) for batch, m, n, dtype in EVERY_ORTHO_TILE if dtype in dtypes))
+        assert len(reached) > 12 and reached <= tested, reached - tested
+
+
+def test_tiles_refuse(hip_lib):
+    for make in (lambda: GatedFfn(8, 8).tiles(0), lambda: GatedFfn(8, 8).tiles(4, compute_units=0), lambda: Orthogonalizer(8, 8, batch=0).tiles(),
+                 lambda: Orthogonalizer(8, 8).tiles(compute_units=0), lambda: GatedFfn(0, 8).tiles(4), lambda: Orthogonalizer(8, 0).tiles()):
+        with pytest.raises(HipError) as err:
+            make()
+        assert err.value.status == hip.RL_ERR_INVALID_ARG

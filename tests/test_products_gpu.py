@@ -152,6 +152,38 @@ def test_every_tile(device, T, D, F, dtype):
     b.check_grads()
 
 
+# The same where it takes more work: every 31st token and feature is worked out in 64 bits, which is some of every tile.
+EVERY_TILE_SAMPLED = [(6906, 4148, 113, "bf16"), (11211, 377, 5573, "fp16"), (650, 8708, 332, "fp16"), (3006, 9557, 668, "bf16"),
+                      (2780, 11071, 148, "fp32"), (1508, 6138, 367, "fp32"), (3062, 749, 5255, "fp32"), (2524, 763, 14052, "fp32"),
+                      (2973, 15814, 989, "fp32"), (13809, 1832, 494, "fp32"), (13932, 1560, 1140, "fp32"), (3161, 14511, 608, "fp32")]
+
+
+@pytest.mark.parametrize("T,D,F,dtype", EVERY_TILE_SAMPLED)
+def test_every_tile_sampled(device, T, D, F, dtype):
+    rng = np.random.default_rng([T, D, F])
+    mat = lambda r, c, s: Matrix(s * rng.standard_normal((r, c), np.float32), dtype)
+    x, dy, wg, wu, wd = mat(T, D, 1.0), mat(T, D, 1.0), mat(F, D, D ** -0.5), mat(F, D, D ** -0.5), mat(D, F, F ** -0.5)
+    op = GatedFfn(D, F, dtype, "silu")
+    y, dx, dwg, dwu, dwd = [Matrix(None, dtype, shape=s) for s in ((T, D), (T, D), (F, D), (F, D), (D, F))]
+    saved, ws = room(op.saved_bytes(T)), room(op.workspace_bytes(T, backward=True))
+    op.forward(x.ptr, wg.ptr, wu.ptr, wd.ptr, y.ptr, T, saved=saved, workspace=ws)
+    op.backward(dy.ptr, x.ptr, wg.ptr, wu.ptr, wd.ptr, saved, dx.ptr, dwg.ptr, dwu.ptr, dwd.ptr, T, workspace=ws)
+    hip.synchronize()
+
+    def close(name, got, want):
+        off = np.abs(got - want[0]) / want[1]
+        assert (off <= 1).all(), f"{name} off by {np.max(off)} bounds"
+
+    ts, fs = np.arange(T)[T % 31::31], np.arange(F)[F % 31::31]
+    rows = po.FeedForward(x.values[ts], wg.values, wu.values, wd.values, "silu", dtype)
+    close("y", y.get()[ts], (rows.y, rows.y_bound))
+    close("dx", dx.get()[ts], rows.backward(dy.values[ts])["dx"])
+    some = po.FeedForward(x.values, wg.values[fs], wu.values[fs], wd.values[:, fs], "silu", dtype).backward(dy.values)
+    close("dw_gate", dwg.get()[fs], some["dw_gate"])
+    close("dw_up", dwu.get()[fs], some["dw_up"])
+    close("dw_down", dwd.get()[:, fs], some["dw_down"])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("T", [5, 40, 150])
 @pytest.mark.parametrize("pad,shift,pad_up", [(8, 0, 24), (3, 1, 3), (0, 5, 0), (16, 8, 9)])
@@ -300,6 +332,23 @@ def test_orthogonalise(device, dtype, batch, rows, cols):
     for i in range(batch):
         want = po.orthogonalise(G[i])
         assert np.linalg.norm(got[i] - want) <= po.orthogonalise_tolerance(G[i], dtype, want)
+
+
+# As EVERY_TILE; fp16 and fp32 go the same way.  A large stack holds two matrices in turn.
+EVERY_ORTHO_TILE = [(1, 32, 35, "bf16"), (40, 392, 482, "bf16"), (40, 259, 268, "bf16"), (40, 590, 647, "bf16"), (1, 32, 996, "bf16"), (40, 410, 71, "bf16"),
+                    (40, 67, 779, "bf16"), (16, 331, 4075, "bf16"), (8, 5248, 907, "bf16"),
+                    (1, 42, 32, "fp16"), (40, 257, 274, "fp32"), (40, 385, 398, "fp16"), (40, 639, 595, "fp32"), (2, 1003, 983, "fp32"), (1, 340, 33, "fp16"),
+                    (1, 996, 1059, "fp16"), (8, 1997, 907, "fp32"), (1, 1708, 2444, "fp16"), (1, 2828, 3029, "fp32")]
+
+
+@pytest.mark.parametrize("batch,rows,cols,dtype", EVERY_ORTHO_TILE)
+def test_orthogonalise_every_tile(device, batch, rows, cols, dtype):
+    two = gradient(np.random.default_rng([batch, rows, cols]), min(batch, 2), rows, cols)
+    got, G = ortho(two[np.arange(batch) % 2], dtype)
+    for i in range(len(two)):
+        want = po.orthogonalise(G[i])
+        allowed = po.orthogonalise_tolerance(G[i], dtype, want)
+        assert np.max(np.linalg.norm(got[i::2] - want, axis=(1, 2))) <= allowed
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
