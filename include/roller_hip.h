@@ -321,10 +321,11 @@ int rl_ffn_backward(const rl_ffn_config* cfg, const void* dy, int lddy, const vo
                     int lddx, void* dw_gate, int ldd_gate, void* dw_up, int ldd_up, void* dw_down, int ldd_down, int T,
                     void* workspace, size_t workspace_bytes, rl_stream stream);
 
-/* The tile of a matrix product and the number of workgroups that share the K steps of each. */
+/* The tile of a matrix product, and how its K steps are shared out: `whole` tiles have a workgroup each, every
+ * other one has `splits`. */
 typedef struct rl_product_tile {
   int rows, cols; /* of the product (gate and up columns count both) */
-  int splits;
+  int splits, whole;
 } rl_product_tile;
 
 /* What the products of a block of T tokens run with on a device of `compute_units` CUs (host arithmetic, no

@@ -134,7 +134,8 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
   } else if (!c.saved) {
     r.h = (T*)room.take((size_t)c.T * s.pitch * ES);
   }
-  if (!r.few) {
+  // (with 17 to 64 tokens the same room whatever the alignment, which a query does not know)
+  if (c.T > FEW) {
     const bool pack = c.T > FEW_ODD;
     r.x = pack_space(room, c.T, c.D, pack && (unaligned || !aligned(c.x)));
     r.w_gate = pack_space(room, c.F, c.D, pack && (unaligned || !aligned(c.w_gate)));

@@ -65,7 +65,7 @@ int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream,
   typedef Shape<T, t::BM, t::BN, t::WM, t::WN, A_KM, B_KM, GATED, SEGS, SYM, t::PER_CU, MI, t::BUFS> S;
   static_assert(t::BM == kTiles[K].bm && t::BN == kTiles[K].bn, "the plan's tiles");
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
-  const long groups = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * p.splits * batch;
+  const long tiles = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch, groups = p.whole + (tiles - p.whole) * p.splits;
   if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
   return launch<tile_kernel<S, Epi>>(what, dim3((unsigned)groups), S::NT, stream, p, epi);
 }
@@ -90,6 +90,7 @@ constexpr int tiles_end() { return A_KM && B_KM && !SYM && SEGS == 1 ? kFewRowsT
 inline int take_plan(Problem& p, const Plan& plan, void* room, Arrivals& arrivals, hipStream_t stream) {
   p.splits = plan.splits;
   p.steps_per_split = plan.steps_per_split;
+  p.whole = plan.whole;
   p.pieces = (float*)room;
   p.arrivals = arrivals.set[arrivals.turn];
   arrivals.turn ^= 1;

@@ -243,8 +243,6 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
   constexpr int PER = 16 / sizeof(T), W = GATED ? 2 : 1, UNROLL = BLOCKS == 1 ? 8 : BLOCKS == 2 ? 4 : 2, ROWS = 16 / PARTS;
   const int waves = blockDim.x / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lr = lane & 15, lg = lane >> 4;
-  const int part_k = (K + PARTS * 4 * PER - 1) / (PARTS * 4 * PER) * (4 * PER);   // whole loads
-  const int from = lr / ROWS * part_k, end = from + part_k < K ? from + part_k : K;
   const int n0 = blockIdx.x * ROWS, row = n0 + lr % ROWS < N ? n0 + lr % ROWS : N - 1;   // (a row past the end is not stored)
   const T* wr[2] = {w0 + (long)row * ldw0, GATED ? w1 + (long)row * ldw1 : nullptr};
   typedef typename x_type<T, SPLIT>::type X;
@@ -261,20 +259,21 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) acc[w][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // the waves take turns at groups of UNROLL x 64 bytes of every part
-  constexpr int GROUP = UNROLL * 4 * PER, XV = SPLIT ? 2 : 1;   // XV: 16-byte loads per chunk of x
-  for (int k0 = wave * GROUP; k0 < part_k; k0 += waves * GROUP) {
+  // the waves take turns at groups of UNROLL x PARTS x 64 bytes
+  constexpr int GROUP = UNROLL * PARTS * 4 * PER, XV = SPLIT ? 2 : 1;   // XV: 16-byte loads per chunk of x
+  const int part = (lr / ROWS * 4 + lg) * PER;
+  for (int k0 = wave * GROUP; k0 < K; k0 += waves * GROUP) {
     v4u wv[W][UNROLL], xv[BLOCKS][UNROLL][XV];
-    const bool whole = k0 + GROUP <= part_k && (PARTS - 1) * part_k + k0 + GROUP <= K;
+    const bool whole = k0 + GROUP <= K;
 #pragma unroll
     for (int t = 0; t < UNROLL; ++t) {
-      const int k = from + k0 + (t * 4 + lg) * PER;
+      const int k = k0 + t * (PARTS * 4 * PER) + part;
 #pragma unroll
-      for (int w = 0; w < W; ++w) wv[w][t] = whole ? whole_chunk(wr[w] + k) : chunk_at(wr[w], k, end);
+      for (int w = 0; w < W; ++w) wv[w][t] = whole ? whole_chunk(wr[w] + k) : chunk_at(wr[w], k, K);
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-        for (int v = 0; v < XV; ++v) xv[b][t][v] = whole ? whole_chunk(xr[b] + k + 4 * v) : chunk_at(xr[b], k + 4 * v, end);
+        for (int v = 0; v < XV; ++v) xv[b][t][v] = whole ? whole_chunk(xr[b] + k + 4 * v) : chunk_at(xr[b], k + 4 * v, K);
     }
 #pragma unroll
     for (int t = 0; t < UNROLL; ++t)

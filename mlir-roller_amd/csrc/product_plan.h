@@ -20,6 +20,7 @@ struct TileCost {
   float step32, fixed32, once32;   // 32-bit operands
 };
 
+constexpr int XCDS = 8;
 constexpr int kFewRowsTile = 4;   // for products of K-major operands only
 constexpr TileCost kTiles[] = {
     {256, 256, 0.967f, 9.5f, 0.0f, 6.886f, 10.0f, 0.0f},
@@ -38,6 +39,7 @@ constexpr size_t kMaxPieces = (size_t)1 << 29;
 struct Plan {
   float time;   // microseconds, by the model
   int tile, splits, steps_per_split;
+  int whole;    // tiles that are not split, all of them if splits is 1
   size_t piece_bytes;
 };
 
@@ -51,21 +53,22 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
     const long nbm = ((long)M_out + c.bm - 1) / c.bm, nbn = ((long)N_out + out_n - 1) / out_n;
     const long tiles = (sym ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch;
     const float step = elem_bytes == 2 ? c.step16 : c.step32, fixed = elem_bytes == 2 ? c.fixed16 : c.fixed32, once = elem_bytes == 2 ? c.once16 : c.once32;
+    // All tiles split alike; or those of full rounds whole, and only what would be a last, partly filled round
+    // shared out over the CUs.
+    const long rounds = tiles / compute_units * compute_units;
     for (int splits = 1; splits <= max_splits; splits *= 2) {
       const int per = (steps + splits - 1) / splits;
       // (every split has two steps at least; the largest tile is not split)
       if (splits > 1 && (t == 0 || per < 2 || (long)(splits - 1) * per >= steps)) break;
-      const size_t pieces = splits > 1 ? (size_t)tiles * splits * c.bm * c.bn * 4 : 0;
-      if (splits > 1 && (pieces > kMaxPieces || tiles > kMaxArrivals)) break;
-      const long per_cu = (tiles * splits + compute_units - 1) / compute_units;
-      float time = once + per_cu * (per * step + fixed);
-      if (splits > 1) time += kJoinFixed + 2.0f * pieces / kPieceBytes;
-      if (best.time == 0.0f || time < best.time) {
-        best.time = time;
-        best.tile = t;
-        best.splits = splits;
-        best.steps_per_split = per;
-        best.piece_bytes = pieces;
+      for (int tail = 0; tail < 2; ++tail) {
+        const long whole = splits == 1 ? tiles : tail ? rounds : 0;
+        if (tail && (splits == 1 || whole == 0 || whole == tiles || compute_units % XCDS != 0)) continue;
+        const size_t pieces = (size_t)(tiles - whole) * splits * c.bm * c.bn * 4;
+        if (pieces > kMaxPieces || tiles - whole > kMaxArrivals) continue;
+        const long alone = (whole + compute_units - 1) / compute_units, shared = ((tiles - whole) * splits + compute_units - 1) / compute_units;
+        float time = once + alone * (steps * step + fixed) + shared * (per * step + fixed);
+        if (splits > 1) time += kJoinFixed + 2.0f * pieces / kPieceBytes;
+        if (best.time == 0.0f || time < best.time) best = {time, t, splits, per, (int)whole, pieces};
       }
     }
   }

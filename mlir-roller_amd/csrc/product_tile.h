@@ -35,6 +35,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include "product_plan.h"
+
 #define PT_DEV static __device__ __forceinline__
 
 namespace product {
@@ -50,7 +52,6 @@ typedef __bf16 bf16_t;
 
 constexpr unsigned OOB = 0x80000000u;   // beyond every resource: a load there returns 0 and touches no memory
 constexpr int STEP_BYTES = 128;         // bytes of k per K step
-constexpr int XCDS = 8;
 
 template <int V>
 struct int_c {
@@ -184,8 +185,9 @@ struct Problem {
   // A tile's K steps may be shared out over workgroups.  Each then leaves its accumulators in `pieces`,
   // and the one that finds the tile's arrival counter at splits - 1 adds them up in split order, whoever
   // that is, so results do not depend on timing.  `arrivals` is zero when the launch starts; the launch
-  // before it on the stream sees to that (clear, n_clear).
-  int splits, steps_per_split;
+  // before it on the stream sees to that (clear, n_clear).  The first `whole` tiles (a multiple of the number of
+  // XCDs) have a workgroup each, the others `splits`.
+  int splits, steps_per_split, whole;
   float* pieces;
   unsigned *arrivals, *clear;
   int n_clear;
@@ -215,6 +217,11 @@ struct Shape {
   static constexpr int A_LOADS = BM * 8 / NT, B_LOADS = BN * 8 / NT;
   static constexpr bool SPLIT = BM * BN <= 192 * 192;   // K steps may be shared out (the registers of 256 x 256 leave no room to)
   static constexpr int OUT_N = GATED ? BN / 2 : BN;   // result columns per tile
+  // Tiles for few rows stream B once.  Groups of neighbours then start at different K steps: rows a power of two
+  // apart would otherwise be read at the same place of a row by everybody at once, which crowds the same memory
+  // channels (24 rows, B of 16384 rows of 8192 bytes, 32 x 64 tiles: 30.9 us, 25.8 with every tile at a step of
+  // its own, 23.6 with every eighth; 4096 rows of 16384 bytes in four splits: 20.0, 17.1, 19.1).
+  static constexpr bool ROTATE = BM <= 64 && A_KM && B_KM && SEGS == 1 && !SYM;
   static_assert(BM % WM == 0 && BN % WN == 0 && WM % MI == 0 && WN % MI == 0, "tile");
   static_assert((BM * 8) % NT == 0 && (BN * 8) % NT == 0, "whole loads per thread");
   static_assert(!GATED || ((WN / 2) % MI == 0 && B_KM), "gate and up halves of a wave tile");
@@ -285,12 +292,20 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
 
   const int nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const int tiles = S::SYM ? nbm * (nbm + 1) / 2 : nbm * nbn;
-  // (grid.x = batch * splits * tiles, in this order: a run of it shares operands)
-  int pid = xcd_order(blockIdx.x, gridDim.x);
-  const int batch = pid / (tiles * p.splits);
-  pid -= batch * tiles * p.splits;
-  const int split = pid / tiles;
-  pid -= split * tiles;
+  // Tiles are numbered through the batch; workgroups are those of the whole tiles, then splits * the other
+  // tiles, in this order: a run of either shares operands.
+  int pid, split = 0;
+  const bool shared = (int)blockIdx.x >= p.whole;
+  if (shared) {
+    const int others = (gridDim.x - p.whole) / p.splits;
+    pid = xcd_order(blockIdx.x - p.whole, gridDim.x - p.whole);
+    split = pid / others;
+    pid += p.whole - split * others;
+  } else {
+    pid = xcd_order(blockIdx.x, p.whole);
+  }
+  const int shared_tile = pid - p.whole, batch = pid / tiles;
+  pid -= batch * tiles;
   int tile_m, tile_n;
   if constexpr (S::SYM) {
     triangle_tile(pid, nbm, tile_m, tile_n);
@@ -305,8 +320,10 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   const int seg_steps = (p.K + S::KSTEP - 1) / S::KSTEP;
   const int first_step = split * p.steps_per_split;
   const int all_steps = seg_steps * S::SEGS;
-  const int last_step = first_step + p.steps_per_split < all_steps ? first_step + p.steps_per_split : all_steps;
+  const int last_step = shared && first_step + p.steps_per_split < all_steps ? first_step + p.steps_per_split : all_steps;
   const int KT = last_step - first_step;
+  // (more rows of tiles share B in the L2, which takes a common start)
+  const int start = S::ROTATE && nbm <= 4 && KT > 0 ? (shared ? tile_n : tile_n / 8) % KT : 0;
 
   // ---- what each lane fetches: offsets from the tile's first element, fixed through the K loop ----
   unsigned a_off[S::A_LOADS], b_off[S::B_LOADS];
@@ -367,6 +384,7 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
     constexpr bool KTEST = decltype(ktest)::value;
     const bool live = kt < KT;
     int step = first_step + (live ? kt : 0), seg = 0;
+    if constexpr (S::ROTATE) step += start < KT - (live ? kt : 0) ? start : start - KT;
     if constexpr (S::SEGS > 1) {
       if (step >= seg_steps) { step -= seg_steps; seg = 1; }
       if constexpr (S::SEGS > 2) {
@@ -492,7 +510,8 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   constexpr int PER = 16 / ES;
   const bool whole = p.K % S::KSTEP == 0 && (S::A_KM || p.M % PER == 0) && (S::B_KM || p.N % PER == 0);
   const bool ragged = p.K % PER != 0;
-  auto is_cut = [&](int kt) __attribute__((always_inline)) { return kt < KT && (first_step + kt + 1) % seg_steps == 0; };
+  const int rotated_cut = last_step == seg_steps ? KT - 1 - start : KT;   // ROTATE: where the last step of K comes
+  auto is_cut = [&](int kt) __attribute__((always_inline)) { return S::ROTATE ? kt == rotated_cut : kt < KT && (first_step + kt + 1) % seg_steps == 0; };
   auto zero_tails = [&](int buf) __attribute__((always_inline)) {
     const int left = p.K % S::KSTEP;
     if (a_k < left && a_k + PER > left) {
@@ -583,7 +602,12 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       if constexpr (BUFS > 3) step(ktest, int_c<3 % BUFS>{}, kt + 3);
       kt += BUFS;
     };
-    if constexpr (S::SEGS == 1) {
+    if constexpr (S::ROTATE) {
+      const int free = whole ? KT : rotated_cut - BUFS;
+      while (kt + BUFS <= KT && kt + BUFS <= free) pass(int_c<0>{});
+      while (kt + BUFS <= KT && kt <= rotated_cut) pass(int_c<1>{});
+      while (kt + BUFS <= KT) pass(int_c<0>{});
+    } else if constexpr (S::SEGS == 1) {
       const int free = whole ? KT : seg_steps - 1 - first_step - BUFS;   // passes that end at or before it
       while (kt + BUFS <= KT && kt + BUFS <= free) pass(int_c<0>{});
       while (kt + BUFS <= KT) pass(int_c<1>{});
@@ -607,9 +631,9 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   __syncthreads();   // the K loop is done with the LDS
 
   // ---- a shared tile: leave the accumulators, and the last one in adds them up ----
-  if constexpr (S::SPLIT) if (p.splits > 1) {
+  if constexpr (S::SPLIT) if (shared) {
     constexpr int QUADS = REGS / 4;
-    const long tile = (long)batch * tiles + pid;
+    const long tile = shared_tile;
     float* const pieces = p.pieces + tile * p.splits * (S::BM * S::BN);
     {
       const __amdgpu_buffer_rsrc_t mine = __builtin_amdgcn_make_buffer_rsrc(pieces + (long)split * (S::BM * S::BN), 0, S::BM * S::BN * 4, 0x00020000);

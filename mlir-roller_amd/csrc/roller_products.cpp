@@ -74,7 +74,7 @@ int check_tokens(int T) {
 
 FfnType type_of(int dtype) { return dtype == RL_F32 ? rl_ffn_f32() : dtype == RL_F16 ? rl_ffn_f16() : rl_ffn_bf16(); }
 
-rl_product_tile tile_of(const product::Plan& p) { return {product::kTiles[p.tile].bm, product::kTiles[p.tile].bn, p.splits}; }
+rl_product_tile tile_of(const product::Plan& p) { return {product::kTiles[p.tile].bm, product::kTiles[p.tile].bn, p.splits, p.whole}; }
 
 #define TRY(expr)          \
   do {                     \

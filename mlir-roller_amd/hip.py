@@ -78,7 +78,7 @@ class OrthoConfig(C.Structure):
 
 class ProductTile(C.Structure):
     """``rl_product_tile``: the tile of a matrix product and its split."""
-    _fields_ = [(n, C.c_int) for n in ("rows", "cols", "splits")]
+    _fields_ = [(n, C.c_int) for n in ("rows", "cols", "splits", "whole")]
 
 
 class StreamKSchedule(C.Structure):

@@ -70,11 +70,11 @@ class GatedFfn:
     PRODUCTS = ("gate and up", "down", "dw_down", "dh", "dx", "dw_gate and dw_up")
 
     def tiles(self, tokens: int, compute_units: int = 256) -> dict:
-        """{product: (tile rows, tile columns, splits)}: what a block of so many tokens runs with (host
+        """{product: (tile rows, tile columns, splits, tiles not split)}: what a block of so many tokens runs with (host
         arithmetic, no device)."""
         out = (ProductTile * 6)()
         check(lib().rl_ffn_tiles(self._at, tokens, compute_units, out))
-        return {name: (t.rows, t.cols, t.splits) for name, t in zip(self.PRODUCTS, out)}
+        return {name: (t.rows, t.cols, t.splits, t.whole) for name, t in zip(self.PRODUCTS, out)}
 
     def forward(self, x, w_gate, w_up, w_down, y, tokens: int, *, ldx: Optional[int] = None, ld_gate: Optional[int] = None,
                 ld_up: Optional[int] = None, ld_down: Optional[int] = None, ldy: Optional[int] = None, saved=None,
@@ -133,10 +133,10 @@ class Orthogonalizer:
     PRODUCTS = ("X X^T", "A A", "B X")
 
     def tiles(self, compute_units: int = 256) -> dict:
-        """{product: (tile rows, tile columns, splits)} of one step (host arithmetic, no device)."""
+        """{product: (tile rows, tile columns, splits, tiles not split)} of one step (host arithmetic, no device)."""
         out = (ProductTile * 3)()
         check(lib().rl_ortho_tiles(self._at, compute_units, out))
-        return {name: (t.rows, t.cols, t.splits) for name, t in zip(self.PRODUCTS, out)}
+        return {name: (t.rows, t.cols, t.splits, t.whole) for name, t in zip(self.PRODUCTS, out)}
 
     def launch(self, G, O, *, ldg: Optional[int] = None, ldo: Optional[int] = None, stride_g: Optional[int] = None,
                stride_o: Optional[int] = None, stream=None, workspace=None, workspace_bytes: Optional[int] = None) -> None:

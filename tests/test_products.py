@@ -129,8 +129,8 @@ def test_dtypes_and_activations_match_the_header():
 
 
 def kinds(tiles):
-    """(product, tile rows, split or not) of every product in the result of tiles()."""
-    return {(name, rows, splits > 1) for name, (rows, _, splits) in tiles.items()}
+    """(product, tile rows, tiles split: none, all, or those after the whole ones) of every product in the result of tiles()."""
+    return {(name, rows, "none" if splits == 1 else "some" if whole else "all") for name, (rows, _, splits, whole) in tiles.items()}
 
 
 def test_the_sizes_of_the_gpu_tests_take_every_product_through_every_tile(hip_lib):
