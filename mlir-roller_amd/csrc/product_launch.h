@@ -47,18 +47,21 @@ inline unsigned blocks_for(long items) {
   return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n);
 }
 
-// Tile k of kTiles (product_plan.h): BM x BN, wave tile, workgroups per CU.
-template <int K>
+// Tile k of kTiles (product_plan.h) for elements of ES bytes: BM x BN, wave tile, workgroups per CU, LDS buffers.
+// Three of the 64 x 64 tiles fit a CU with three buffers each, two with four.  With 32 bits, where the matrix units
+// are the limit, three are faster (333 x 5462 x 1001: 39 us, 44 with two); with 16 bits a step is too short for
+// the loads of two (200 x 2880 x 7680: 30 us, 23 with two workgroups and four buffers).
+template <int K, int ES>
 struct tile;
-template <> struct tile<0> { static constexpr int BM = 256, BN = 256, WM = 128, WN = 128, PER_CU = 1, BUFS = 2; };
-template <> struct tile<1> { static constexpr int BM = 192, BN = 192, WM = 96, WN = 96, PER_CU = 1, BUFS = 3; };
-template <> struct tile<2> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 1, BUFS = 4; };
-template <> struct tile<3> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = 2, BUFS = 4; };
-template <> struct tile<4> { static constexpr int BM = 32, BN = 64, WM = 32, WN = 32, PER_CU = 3, BUFS = 4; };
+template <int ES> struct tile<0, ES> { static constexpr int BM = 256, BN = 256, WM = 128, WN = 128, PER_CU = 1, BUFS = 2; };
+template <int ES> struct tile<1, ES> { static constexpr int BM = 192, BN = 192, WM = 96, WN = 96, PER_CU = 1, BUFS = 3; };
+template <int ES> struct tile<2, ES> { static constexpr int BM = 128, BN = 128, WM = 64, WN = 64, PER_CU = 1, BUFS = 4; };
+template <int ES> struct tile<3, ES> { static constexpr int BM = 64, BN = 64, WM = 32, WN = 32, PER_CU = ES == 4 ? 3 : 2, BUFS = ES == 4 ? 3 : 4; };
+template <int ES> struct tile<4, ES> { static constexpr int BM = 32, BN = 64, WM = 32, WN = 32, PER_CU = 3, BUFS = 4; };
 
 template <int K, class T, int A_KM, int B_KM, int GATED, int SEGS, int SYM, class Epi>
 int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream, const char* what) {
-  typedef tile<K> t;
+  typedef tile<K, sizeof(T)> t;
   // Blocks of 32 x 32, or of 16 x 16 where 32 do not fit: gated wave tiles of 32 or 96 columns are 16 or 48 of
   // each kind, and the few-rows tile has two blocks of 16 rows.
   constexpr int MI = K == kFewRowsTile || (GATED && t::WN / 2 % 32 != 0) ? 16 : 32;

@@ -8,9 +8,10 @@
 namespace product {
 
 // What a tile costs on one compute unit, in microseconds: `step` per K step of 128 bytes, `fixed` for first
-// loads and epilogue, `once` for the launch.  Fitted to 840 timed products (64 to 5800 rows, 64 to 11000
-// columns, K 64 to 12000; K-major and row-major operands; 1 to 8 splits): the model is off by 4 to 13 % rms,
-// and what it chooses is on average 0.2 % slower, at worst 6 %, than the fastest choice timed.
+// loads and epilogue, `once` for the launch.  Fitted to 3588 timed products (32 to 8192 rows, 64 to 11000
+// columns, K 64 to 11000, operands out of memory; K-major and row-major operands; whole tiles, all split, the
+// last round split): the model is off by 13 % (16 bits) and 7 % (32 bits) rms, and what it chooses is on average
+// 1 %, at worst 19 %, slower than the fastest choice timed.
 // The large tiles have the higher rate where they fill the CUs (4096^3 in bf16: 103 us with 256 x 256 tiles,
 // 113 with 192, 120 with 128, 191 with 64); the small ones where the others would not (1024 x 1920 x 5000:
 // 118, 65, 49 and 46 us unsplit), and 192 x 192 makes the lower triangle of 4096 x 4096 253 tiles for 256 CUs.
@@ -23,14 +24,15 @@ struct TileCost {
 constexpr int XCDS = 8;
 constexpr int kFewRowsTile = 4;   // for products of K-major operands only
 constexpr TileCost kTiles[] = {
-    {256, 256, 0.967f, 9.5f, 0.0f, 6.886f, 10.0f, 0.0f},
-    {192, 192, 0.554f, 7.6f, 0.0f, 3.872f, 7.8f, 0.0f},
-    {128, 128, 0.316f, 4.6f, 0.3f, 1.740f, 4.9f, 0.0f},
-    {64, 64, 0.159f, 1.0f, 2.8f, 0.448f, 1.2f, 2.4f},
-    {32, 64, 0.120f, 1.0f, 2.6f, 0.420f, 1.2f, 2.4f},
+    {256, 256, 0.957f, 8.8f, 0.0f, 6.879f, 8.5f, 0.0f},
+    {192, 192, 0.598f, 7.9f, 0.0f, 3.940f, 7.6f, 0.8f},
+    {128, 128, 0.340f, 5.1f, 0.0f, 1.748f, 4.5f, 0.8f},
+    {64, 64, 0.175f, 1.0f, 2.6f, 0.439f, 0.8f, 2.4f},
+    {32, 64, 0.138f, 0.5f, 3.3f, 0.414f, 0.0f, 3.9f},
 };
-constexpr float kJoinFixed = 2.0f;          // what splitting a tile costs the one that adds it up, microseconds
-constexpr float kPieceBytes = 3.5e6f;       // bytes of pieces written or read per microsecond
+// What splitting costs, microseconds: the workgroup that adds a tile up waits once for every piece ...
+constexpr float kJoinPiece = 0.55f;
+constexpr float kPieceBytes = 4.0e6f;       // ... and the pieces are written and read, so many bytes per microsecond
 constexpr float kClearLaunch = 3.0f;        // a launch that clears the arrival counters, where no other does
 constexpr int kMaxSplits = 16;
 constexpr int kMaxArrivals = 4096;          // tiles of a split product
@@ -67,7 +69,7 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
         if (pieces > kMaxPieces || tiles - whole > kMaxArrivals) continue;
         const long alone = (whole + compute_units - 1) / compute_units, shared = ((tiles - whole) * splits + compute_units - 1) / compute_units;
         float time = once + alone * (steps * step + fixed) + shared * (per * step + fixed);
-        if (splits > 1) time += kJoinFixed + 2.0f * pieces / kPieceBytes;
+        if (splits > 1) time += kJoinPiece * splits + 2.0f * pieces / kPieceBytes;
         if (best.time == 0.0f || time < best.time) best = {time, t, splits, per, (int)whole, pieces};
       }
     }

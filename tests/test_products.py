@@ -129,8 +129,9 @@ def test_dtypes_and_activations_match_the_header():
 
 
 def kinds(tiles):
-    """(product, tile rows, tiles split: none, all, or those after the whole ones) of every product in the result of tiles()."""
-    return {(name, rows, "none" if splits == 1 else "some" if whole else "all") for name, (rows, _, splits, whole) in tiles.items()}
+    """Of every product in the result of tiles(): (product, tile rows, some are split), and where that is only those after
+    the whole ones, (tile rows,)."""
+    return {(name, rows, splits > 1) for name, (rows, _, splits, whole) in tiles.items()} | {(rows,) for rows, _, splits, whole in tiles.values() if splits > 1 and whole}
 
 
 def test_the_sizes_of_the_gpu_tests_take_every_product_through_every_tile(hip_lib):
@@ -138,8 +139,9 @@ def test_the_sizes_of_the_gpu_tests_take_every_product_through_every_tile(hip_li
     from test_products_gpu import EVERY_ORTHO_TILE, EVERY_TILE, EVERY_TILE_SAMPLED
     pick = random.Random(1)
     between = lambda lo, hi: int(2 ** pick.uniform(lo, hi))
-    for dtypes in (("bf16", "fp16"), ("fp32",)):
-        reached = set().union(*(kinds(GatedFfn(between(6, 14), between(6, 14), dtypes[0]).tiles(between(5, 14))) for _ in range(4000)))
+    for dtypes, most in ((("bf16", "fp16"), 1e15), (("fp32",), 4e10)):        # (T D F; in fp32 what lies beyond would take minutes)
+        sizes = [(between(5, 14), between(6, 14), between(6, 14)) for _ in range(4000)]
+        reached = set().union(*(kinds(GatedFfn(D, F, dtypes[0]).tiles(T)) for T, D, F in sizes if T * D * F <= most))
         tested = set().union(*(kinds(GatedFfn(D, F, dtype).tiles(T)) for T, D, F, dtype in EVERY_TILE + EVERY_TILE_SAMPLED if dtype in dtypes))
         assert len(reached) > 25 and reached <= tested, reached - tested
     for dtypes in (("bf16",), ("fp16", "fp32")):

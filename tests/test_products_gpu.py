@@ -155,7 +155,9 @@ def test_every_tile(device, T, D, F, dtype):
 # The same where it takes more work: every 31st token and feature is worked out in 64 bits, which is some of every tile.
 EVERY_TILE_SAMPLED = [(6906, 4148, 113, "bf16"), (11211, 377, 5573, "fp16"), (650, 8708, 332, "fp16"), (3006, 9557, 668, "bf16"),
                       (2780, 11071, 148, "fp32"), (1508, 6138, 367, "fp32"), (3062, 749, 5255, "fp32"), (2524, 763, 14052, "fp32"),
-                      (2973, 15814, 989, "fp32"), (13809, 1832, 494, "fp32"), (13932, 1560, 1140, "fp32"), (3161, 14511, 608, "fp32")]
+                      (2973, 15814, 989, "fp32"), (13809, 1832, 494, "fp32"), (13932, 1560, 1140, "fp32"), (3161, 14511, 608, "fp32"),
+                      (1651, 10892, 1021, "bf16"), (32, 1424, 8803, "fp16"), (4667, 79, 1889, "fp32"), (641, 80, 753, "fp32"), (654, 1512, 82, "fp32"),
+                      (2315, 88, 641, "fp32"), (549, 897, 9763, "fp32"), (32, 364, 8746, "fp32")]
 
 
 @pytest.mark.parametrize("T,D,F,dtype", EVERY_TILE_SAMPLED)
@@ -190,6 +192,20 @@ def test_every_tile_sampled(device, T, D, F, dtype):
 def test_leading_dimensions_and_alignment(device, dtype, T, pad, shift, pad_up):
     b = Block(T, 96, 136, dtype, "silu", pad=pad, shift=shift, pad_up=pad_up)
     saved = room(b.op.saved_bytes(T))
+    b.forward(saved)
+    b.check_y()
+    b.backward(saved)
+    b.check_grads()
+
+
+@pytest.mark.parametrize("T", [17, 40, 64, 65])
+def test_odd_extents_with_even_leading_dimensions(device, T):
+    # rows of 65 and 33 elements, 72 and 40 apart: the workspace that a query without leading dimensions asks for does
+    b = Block(T, 65, 33, "bf16", "silu", pad=7)
+    b.unaligned = False
+    saved = room(b.op.saved_bytes(T))
+    b.forward()
+    b.check_y()
     b.forward(saved)
     b.check_y()
     b.backward(saved)
@@ -336,9 +352,11 @@ def test_orthogonalise(device, dtype, batch, rows, cols):
 
 # As EVERY_TILE; fp16 and fp32 go the same way.  A large stack holds two matrices in turn.
 EVERY_ORTHO_TILE = [(1, 32, 35, "bf16"), (40, 392, 482, "bf16"), (40, 259, 268, "bf16"), (40, 590, 647, "bf16"), (1, 32, 996, "bf16"), (40, 410, 71, "bf16"),
-                    (40, 67, 779, "bf16"), (16, 331, 4075, "bf16"), (8, 5248, 907, "bf16"),
+                    (40, 67, 779, "bf16"), (16, 331, 4075, "bf16"), (8, 5248, 907, "bf16"), (19, 325, 5164, "bf16"), (26, 888, 206, "bf16"), (52, 782, 637, "bf16"),
+                    (1, 1066, 998, "bf16"), (2, 967, 1233, "bf16"), (52, 1712, 899, "bf16"), (10, 1754, 1742, "bf16"),
                     (1, 42, 32, "fp16"), (40, 257, 274, "fp32"), (40, 385, 398, "fp16"), (40, 639, 595, "fp32"), (2, 1003, 983, "fp32"), (1, 340, 33, "fp16"),
-                    (1, 996, 1059, "fp16"), (8, 1997, 907, "fp32"), (1, 1708, 2444, "fp16"), (1, 2828, 3029, "fp32")]
+                    (1, 996, 1059, "fp16"), (8, 1997, 907, "fp32"), (1, 1708, 2444, "fp16"), (1, 2828, 3029, "fp32"), (26, 888, 206, "fp16"), (52, 782, 637, "fp32"),
+                    (59, 558, 456, "fp32")]
 
 
 @pytest.mark.parametrize("batch,rows,cols,dtype", EVERY_ORTHO_TILE)
