@@ -270,9 +270,10 @@ int rl_gemm_f32(const rl_gemm_config* cfg, const float* A, const float* B, float
  * Not in the reference, which stops at one fp32 product (src/roller.py:62).  These run on kernels that are
  * compiled with the library (no JIT at run time) and follow its conventions: status and text, device
  * pointers, one device, NULL = the default stream, everything enqueued and nothing waited for.
- * Matrices are row-major with a leading dimension in elements >= their columns; any alignment and any
- * leading dimension is accepted, rows of whole aligned 16-byte chunks are fastest (others are copied into
- * the workspace by the call, with more than 64 tokens).
+ * Matrices are row-major with a leading dimension in elements >= their columns; any element
+ * alignment and any leading dimension is accepted.  Rows that start at whole 128-byte lines are fastest; 16-bit
+ * rows that start at odd elements are copied into the workspace by the call (backward, and forward with more
+ * than 64 tokens).
  *
  * Workspace: the caller's (256-byte aligned, at least what the *_workspace_bytes function says; contents
  * do not matter before or after; calls that share one must not overlap on the device), or NULL for one
@@ -298,9 +299,10 @@ typedef struct rl_ffn_config {
   int d_model, d_ff;
 } rl_ffn_config;
 
-/* Workspace of a forward call of T tokens, and with `backward` the larger of that and a backward call's.
- * `unaligned`: room for packed copies although d_model and d_ff are whole 16-byte chunks (pointers or
- * leading dimensions that are not). */
+/* Workspace of a forward call of T tokens, and with `backward` the larger of that and a backward call's.  It
+ * counts packed copies where dense 16-bit rows would start at odd elements; `unaligned` counts them in any
+ * case: for 16-bit pointers or leading dimensions that are odd although d_model and d_ff are even, and for a
+ * backward call whose gate and up weights have different leading dimensions. */
 int rl_ffn_workspace_bytes(const rl_ffn_config* cfg, int T, int backward, int unaligned, size_t* bytes);
 
 /* Size of what a forward call keeps for the backward pass: x Wg^T and x Wu^T in fp32, their gated product

@@ -193,8 +193,10 @@ __global__ __launch_bounds__(256) void zero_kernel(T* c, int ld, int rows, int c
 //
 // PARTS = 2 or 4: with few tokens the 16 x 16 block of an MFMA holds that many parts of K side by side, part q in
 // rows and columns 16 / PARTS * q and on; of the products of all parts with all parts only the diagonal blocks
-// are used.  A workgroup then owns fewer weight rows, and there are more of them (1024 rows: 64 workgroups of
-// 16 rows for 256 CUs, or 256 of 4: 8.9 us against PARTS_US us).
+// are used.  A workgroup then owns fewer weight rows, and there are more of them (1024 rows of 4096 elements: 64
+// workgroups of 16 rows for 256 CUs, or 256 of 4: 8.9 us against 4.7).  The parts are 64-byte pieces that lie side
+// by side, so a load takes 128 or 256 bytes of a row: one token, weights of 4096 x 12288, 57 us; with the
+// quarters of K as parts, 64.
 //
 // Rows may start at any element: a chunk is loaded whole, at the alignment of its type, and the last one of a
 // row element by element.

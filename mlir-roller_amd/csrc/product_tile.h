@@ -492,9 +492,9 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   // two rounds.  A quarter into the last round the step's own reads are over and kt + 1 must have landed:
   // the workgroup meets, reads the first fragments of kt + 1 and sends the first loads of kt + BUFS into
   // `cur`.
-  // The order of instructions is the order written here (sched_barrier between the slots, one MFMA each, four with 32-bit operands):
-  // reads and loads are spread over the MFMAs, which run meanwhile; issued in a bunch they hold up the
-  // MFMAs behind them.
+  // The order of instructions is the order written here (sched_barrier between the slots, one MFMA each, four
+  // with 32-bit operands): reads and loads are spread over the MFMAs, which run meanwhile; issued in a bunch
+  // they hold up the MFMAs behind them.
   constexpr int PARTS = mma<T, MI>::PER_FRAG, G = TM * TN, FRAGS = TM + TN, L = S::A_LOADS + S::B_LOADS;
   constexpr int BUFS = S::BUFS, EARLY = G / 4, TAIL = L * S::TAIL_LOADS / 4;
   auto slot_mfma = [&](const frags& f, int t) __attribute__((always_inline)) {

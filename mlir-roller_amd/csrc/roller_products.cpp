@@ -100,7 +100,7 @@ int ProductRoom::take(hipStream_t stream, void* user, size_t user_bytes, size_t 
   *out = nullptr;
   if (user) {
     if ((uintptr_t)user % 256) return rl_fail(RL_ERR_INVALID_ARG, "%s: the workspace must be 256-byte aligned", what);
-    if (user_bytes < need) return rl_fail(RL_ERR_INVALID_ARG, "%s: this call needs a workspace of %zu bytes, got %zu (rows that are not whole 16-byte chunks need room for a packed copy)", what, need, user_bytes);
+    if (user_bytes < need) return rl_fail(RL_ERR_INVALID_ARG, "%s: this call needs a workspace of %zu bytes, got %zu (16-bit rows at odd elements, and backward gate and up weights with different leading dimensions, need room for a packed copy)", what, need, user_bytes);
     *out = (char*)user;
     return RL_OK;
   }
@@ -170,8 +170,8 @@ int rl_ffn_workspace_bytes(const rl_ffn_config* cfg, int T, int backward, int un
     c.F = cfg->d_ff;
     const FfnType t = type_of(cfg->dtype);
     if (T == 0) return RL_OK;
-    // (no pointers here, and leading dimensions that are those of dense rows: packed copies are counted for
-    // rows that are not whole 16-byte chunks, or for all with `unaligned`)
+    // (no pointers here, and leading dimensions that are those of dense rows: packed copies are counted where
+    // such rows start at odd elements, or for all with `unaligned`)
     c.x.ld = c.w_gate.ld = c.w_up.ld = c.dy.ld = c.D;
     c.w_down.ld = c.F;
     size_t need = t.forward_room(c, unaligned != 0);

@@ -55,7 +55,8 @@ class GatedFfn:
 
     def workspace_bytes(self, tokens: int, backward: bool = False, unaligned: bool = False) -> int:
         """Workspace of a forward call (with ``backward``: enough for both passes).  ``unaligned``: for
-        pointers or leading dimensions that are not multiples of 16 bytes although the extents are."""
+        16-bit rows that start at odd elements although the extents are even, and for a backward call whose
+        gate and up weights have different leading dimensions."""
         hip.init()
         out = C.c_size_t()
         check(lib().rl_ffn_workspace_bytes(self._at, tokens, int(backward), int(unaligned), C.byref(out)))

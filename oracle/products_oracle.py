@@ -135,7 +135,7 @@ def orthogonalise_tolerance(G: np.ndarray, dtype: str, exact: np.ndarray, **how)
 
     The iteration multiplies errors by up to 3.4 in every step, so a worst-case bound says nothing; but the
     roundings are many and independent, and their sum over a matrix has a sharp norm.  A model with the
-    library's roundings in 64-bit arithmetic (fp16 operands scaled by 2^8 and fp32 for the rest where the
+    library's roundings in 64-bit arithmetic (fp16 operands scaled by 2^9 and fp32 for the rest where the
     matrices are bf16; where they are fp16 or fp32, operands of 21 bits: the high and the low part of a
     two-part fp16 number, or more) gives that norm for the matrix at hand; sums of n products in
     fp32 add a random walk of n half steps, at most sqrt(n) 2^-24 of the sum's terms, amplified alike.
@@ -144,7 +144,7 @@ def orthogonalise_tolerance(G: np.ndarray, dtype: str, exact: np.ndarray, **how)
     norm), and half a step of the output."""
     f32 = lambda X: X.astype(np.float32).astype(np.float64)
     if dtype == "bf16":
-        operand = lambda X: (X * 256).astype(np.float16).astype(np.float64) / 256
+        operand = lambda X: (X * 512).astype(np.float16).astype(np.float64) / 512
     else:
         operand = lambda X: np.round(X * 2.0 ** 21 / 2.0 ** np.ceil(np.log2(np.abs(X) + 1e-300))) / 2.0 ** 21 * 2.0 ** np.ceil(np.log2(np.abs(X) + 1e-300))
     model = orthogonalise(G, keep=f32, operand=operand, **how)
