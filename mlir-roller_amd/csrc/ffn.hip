@@ -119,7 +119,7 @@ struct ForwardRoom {
   float* h32;
   char *arrivals, *pieces;
   Plan up, down;
-  bool few;   // takes few_rows_kernel
+  bool few_up, few_down;   // takes few_rows_kernel
   size_t bytes;
 };
 
@@ -127,8 +127,8 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
   Carver room(c.room);
   ForwardRoom r = {};
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
-  const bool odd = !aligned(c.x) || !aligned(c.w_gate) || !aligned(c.w_up) || !aligned(c.w_down);
-  r.few = c.T <= FEW || (c.T <= FEW_ODD && odd);
+  r.few_up = c.T <= FEW || (c.T <= FEW_ODD && !(aligned(c.x) && aligned(c.w_gate) && aligned(c.w_up)));
+  r.few_down = c.T <= FEW || (c.T <= FEW_ODD && !aligned(c.w_down));
   if (c.T <= EXACT_TOKENS) {
     r.h32 = (float*)room.take((size_t)c.T * s.pitch * 4);
   } else if (!c.saved) {
@@ -150,22 +150,24 @@ ForwardRoom forward_carve(const FfnCall& c, bool unaligned) {
   return r;
 }
 
-template <int BLOCKS, int PARTS, int SPLIT, int KIND>
-int few_rows(const FfnCall& c, const void* h, const GatedForward<T, KIND>& gated, const Store<T>& out, const FfnSaved& s) {
-  // Enough waves to keep the memory busy from every CU: up to 16 share the K of a workgroup's rows, none with
-  // fewer than 256 bytes of each part of a row.
-  auto waves = [&](int groups, int K) {
-    int w = 1;
-    while (w < 16 && (long)groups * w < 16L * c.compute_units && K / PARTS * ES >= 512 * w) w *= 2;
-    return 64 * w;
+// A product of few tokens: x (SPLIT: in fp32) with the rows of w0, GATED: and w1.
+template <int GATED, int SPLIT, class Epi>
+int few_rows(const FfnCall& c, const void* x, int ldx, const FfnMatrix& w0, const FfnMatrix& w1, int N, int K, const Epi& epi, const char* what) {
+  auto as = [&](auto blocks, auto parts) -> int {
+    constexpr int BLOCKS = decltype(blocks)::value, PARTS = decltype(parts)::value, ROWS = 16 / PARTS;
+    const int groups = (N + ROWS - 1) / ROWS;
+    // Enough waves to keep the memory busy from every CU: up to 16 share the K of a workgroup's rows, none with
+    // fewer than 256 bytes of each part of a row.
+    int waves = 1;
+    while (waves < 16 && (long)groups * waves < 16L * c.compute_units && K / PARTS * ES >= 512 * waves) waves *= 2;
+    return launch<few_rows_kernel<T, BLOCKS, PARTS, GATED, SPLIT, Epi>>(what, dim3(groups), 64 * waves, c.stream, (const typename x_type<T, SPLIT>::type*)x, ldx, (const T*)w0.p, w0.ld, (const T*)w1.p, w1.ld, c.T,
+                                                                        N, K, epi);
   };
-  constexpr int ROWS = 16 / PARTS;
-  typedef typename x_type<T, SPLIT>::type H;
-  const int up = (c.F + ROWS - 1) / ROWS, down = (c.D + ROWS - 1) / ROWS;
-  PT_TRY(launch<few_rows_kernel<T, BLOCKS, PARTS, 1, 0, GatedForward<T, KIND>>>("ffn: gate and up", dim3(up), waves(up, c.D), c.stream, (const T*)c.x.p, c.x.ld, (const T*)c.w_gate.p, c.w_gate.ld,
-                (const T*)c.w_up.p, c.w_up.ld, c.T, c.F, c.D, gated));
-  return launch<few_rows_kernel<T, BLOCKS, PARTS, 0, SPLIT, Store<T>>>("ffn: down", dim3(down), waves(down, c.F), c.stream, (const H*)h, s.pitch, (const T*)c.w_down.p, c.w_down.ld, (const T*)nullptr, 0, c.T,
-                c.D, c.F, out);
+  if (c.T <= 4) return as(int_c<1>{}, int_c<4>{});
+  if (c.T <= 8) return as(int_c<1>{}, int_c<2>{});
+  if (c.T <= 16) return as(int_c<1>{}, int_c<1>{});
+  if constexpr (SPLIT) return RL_ERR_INTERNAL;   // (no more than EXACT_TOKENS)
+  else return c.T <= 32 ? as(int_c<2>{}, int_c<1>{}) : as(int_c<4>{}, int_c<1>{});
 }
 
 size_t forward_room(const FfnCall& c, bool unaligned) { return forward_carve(c, unaligned).bytes; }
@@ -181,26 +183,26 @@ int forward_as(const FfnCall& call) {
   gated.u = c.saved ? (float*)((char*)c.saved + s.u) : nullptr;
   gated.pitch = s.pitch;
   const Store<T> out = store(c.y, c.ldy, c.D);
-  if (r.few) {
-    gated.h32 = r.h32;
-    constexpr int SPLIT = EXACT_TOKENS != 0;
-    const void* h = r.h32 ? (const void*)r.h32 : gated.h;
-    if (c.T <= 4) return few_rows<1, 4, SPLIT>(c, h, gated, out, s);
-    if (c.T <= 8) return few_rows<1, 2, SPLIT>(c, h, gated, out, s);
-    if (c.T <= 16) return few_rows<1, 1, SPLIT>(c, h, gated, out, s);
-    if (c.T <= 32) return few_rows<2, 1, 0>(c, h, gated, out, s);
-    return few_rows<4, 1, 0>(c, h, gated, out, s);
-  }
-
+  gated.h32 = r.h32;
   PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
   PT_TRY(pack(c.w_gate, c.F, c.D, r.w_gate, c.stream));
   PT_TRY(pack(c.w_up, c.F, c.D, r.w_up, c.stream));
   PT_TRY(pack(c.w_down, c.D, c.F, r.w_down, c.stream));
   Arrivals arrivals = arrivals_at(r.arrivals, false);
-  Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, c.F);
-  up.b[1] = c.w_up.p;
-  up.ldb1 = c.w_up.ld;
-  PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, r.up, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: gate and up")));
+  if (r.few_up) {
+    PT_TRY((few_rows<1, 0>(c, c.x.p, c.x.ld, c.w_gate, c.w_up, c.F, c.D, gated, "ffn: gate and up")));
+  } else {
+    Problem up = problem(c.x.p, c.x.ld, c.w_gate.p, c.w_gate.ld, c.T, c.F, c.D, c.T, c.F);
+    up.b[1] = c.w_up.p;
+    up.ldb1 = c.w_up.ld;
+    PT_TRY((run_product<T, 1, 1, 1, 1, 0>(up, r.up, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: gate and up")));
+  }
+  if (r.few_down) {
+    if constexpr (EXACT_TOKENS != 0) {
+      if (r.h32) return few_rows<0, 1>(c, r.h32, s.pitch, c.w_down, {}, c.D, c.F, out, "ffn: down");
+    }
+    return few_rows<0, 0>(c, gated.h, s.pitch, c.w_down, {}, c.D, c.F, out, "ffn: down");
+  }
   const Problem down = problem(gated.h, s.pitch, c.w_down.p, c.w_down.ld, c.T, c.D, c.F, c.T, c.D);
   return run_product<T, 1, 1, 0, 1, 0>(down, r.down, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: down");
 }

@@ -162,19 +162,34 @@ struct GatedBackward {
 
 // ---- small kernels ----------------------------------------------------------------------------------
 
+// 16 bytes from any element on: loaded whole, at the alignment of their type, and at the end of a row element by
+// element.
+template <class T>
+PT_DEV v4u whole_chunk(const T* at) {
+  v4u v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(at, sizeof(T)), 16);
+  return v;
+}
+template <class T>
+PT_DEV v4u chunk_at(const T* row, int k, int K) {
+  constexpr int PER = 16 / sizeof(T);
+  if (k + PER <= K) return whole_chunk(row + k);
+  typedef T chunk __attribute__((ext_vector_type(PER)));
+  chunk v;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) v[e] = k + e < K ? row[k + e] : (T)0.0f;
+  return __builtin_bit_cast(v4u, v);
+}
+
 // Copies a matrix whose rows are not dword-aligned (16-bit elements at odd places) into one whose rows are,
-// with zeros up to a whole chunk.  One element per access: such rows may start at any address.
+// with zeros up to the pitch.
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* src, int ld, int rows, int cols, T* dst, int pitch) {
   constexpr int PER = 16 / sizeof(T);
-  typedef T chunk __attribute__((ext_vector_type(PER)));
   const int chunks = pitch / PER;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * chunks; i += gridDim.x * 256L) {
     const int r = (int)(i / chunks), c = (int)(i % chunks) * PER;
-    chunk v;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = c + e < cols ? src[(long)r * ld + c + e] : (T)0.0f;
-    *(chunk*)(dst + (long)r * pitch + c) = v;
+    *(v4u*)(dst + (long)r * pitch + c) = chunk_at(src + (long)r * ld, c, cols);
   }
 }
 
@@ -198,25 +213,7 @@ __global__ __launch_bounds__(256) void zero_kernel(T* c, int ld, int rows, int c
 // by side, so a load takes 128 or 256 bytes of a row: one token, weights of 4096 x 12288, 57 us; with the
 // quarters of K as parts, 64.
 //
-// Rows may start at any element: a chunk is loaded whole, at the alignment of its type, and the last one of a
-// row element by element.
-template <class T>
-PT_DEV v4u whole_chunk(const T* at) {
-  v4u v;
-  __builtin_memcpy(&v, __builtin_assume_aligned(at, sizeof(T)), 16);
-  return v;
-}
-template <class T>
-PT_DEV v4u chunk_at(const T* row, int k, int K) {
-  constexpr int PER = 16 / sizeof(T);
-  if (k + PER <= K) return whole_chunk(row + k);
-  typedef T chunk __attribute__((ext_vector_type(PER)));
-  chunk v;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) v[e] = k + e < K ? row[k + e] : (T)0.0f;
-  return __builtin_bit_cast(v4u, v);
-}
-
+// Rows may start at any element (chunk_at).
 //
 // SPLIT: x is fp32 although the weights have 16 bits.  Each of its elements then goes into the product as
 // the sum of two of 16 bits, high part and remainder: twice the matrix instructions, which are idle anyway,
