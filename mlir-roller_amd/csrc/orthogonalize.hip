@@ -157,7 +157,8 @@ struct Gram {
   __device__ __forceinline__ Gram at(int batch) const { return {A.of(batch)}; }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const { A.put(m, n, v * kUnscale, ok); }
+  __device__ __forceinline__ v4f value(int, int, v4f v, In) const { return v * kUnscale; }
+  __device__ __forceinline__ void put(int m, int n, v4f v, bool ok) const { A.put(m, n, v, ok); }
 };
 
 // B = b A + c A^2, from the product of Ao with itself
@@ -171,15 +172,16 @@ struct Polynomial {
     float dm;
   };
   __device__ __forceinline__ In get(int m, int n) const { return {get_operand<PARTS>(A.off + (long)m * A.pitch + n, A.parts), *(const v4f*)(A.diag + n), A.diag[m]}; }
-  __device__ __forceinline__ void put(int m, int n, v4f v, In in, bool ok) const {
+  __device__ __forceinline__ v4f value(int m, int n, v4f v, In in) const {
     v4f x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float sq = v[e] * kUnscale;
       x[e] = m == n + e ? b * in.dm + c * (sq + in.dm * in.dm) : b * in.ao[e] + c * (sq + (in.dm + in.dn[e]) * in.ao[e]);
     }
-    B.put(m, n, x, ok);
+    return x;
   }
+  __device__ __forceinline__ void put(int m, int n, v4f v, bool ok) const { B.put(m, n, v, ok); }
 };
 
 // X <- (a + diag(B)) X + Bo X, in place (every element is read and written by one lane); the last step of a

@@ -3,7 +3,8 @@
 //
 // An epilogue is a struct with at(batch), which picks the buffers of a batch entry, get(m, n), which
 // loads what it needs besides the product, and put(m, n, v, in, ok): four consecutive columns n .. n+3 of row
-// m, n a multiple of 4 (gated products: put(m, n, gate, up, in, ok)), stored if ok.
+// m, n a multiple of 4 (gated products: put(m, n, gate, up, in, ok)), stored if ok.  Of a symmetric product
+// value(m, n, v, in) is what v becomes and put(m, n, value, ok) stores it, once as it is and once mirrored.
 
 #ifndef PRODUCT_OPS_H
 #define PRODUCT_OPS_H

@@ -712,7 +712,7 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
 #pragma unroll
           for (int k = 0; k < BATCH; ++k) {
             const int u = u0 + 64 * k, m = (TR ? nb : mb) + u / PER, n = (TR ? mb : nb) + u % PER * 4;
-            in[k] = out.get(m < m_last ? m : m_last, n < n_last ? n : n_last);
+            if constexpr (!TR) in[k] = out.get(m < m_last ? m : m_last, n < n_last ? n : n_last);
           }
 #pragma unroll
           for (int k = 0; k < BATCH; ++k) {
@@ -721,8 +721,14 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
             const unsigned from = mine + (TR ? c * PITCH + r : r * PITCH + c) * 4;
             if constexpr (S::GATED) {
               out.put(m, n, lds_read<v4f>(from), lds_read<v4f>(from + S::WN / 2 * 4), in[k], ok);
-            } else if constexpr (TR) {
-              out.put(m, n, v4f{lds_read<float>(from), lds_read<float>(from + PITCH * 4), lds_read<float>(from + PITCH * 8), lds_read<float>(from + PITCH * 12)}, in[k], ok);
+            } else if constexpr (S::SYM) {
+              if constexpr (TR) {
+                out.put(m, n, v4f{lds_read<float>(from), lds_read<float>(from + PITCH * 4), lds_read<float>(from + PITCH * 8), lds_read<float>(from + PITCH * 12)}, ok);
+              } else {
+                const v4f v = out.value(m, n, lds_read<v4f>(from), in[k]);
+                lds_write(from, v);
+                out.put(m, n, v, ok);
+              }
             } else {
               out.put(m, n, lds_read<v4f>(from), in[k], ok);
             }
@@ -730,7 +736,8 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
         }
       };
       units(int_c<0>{});
-      // the mirror image of a tile below the diagonal: four rows of one column a unit
+      // the mirror image of a tile below the diagonal, of the values that have just left: four rows of one column
+      // a unit
       if constexpr (S::SYM) {
         if (tile_m != tile_n) units(int_c<1>{});
       }
