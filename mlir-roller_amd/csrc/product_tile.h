@@ -69,10 +69,12 @@ PT_DEV unsigned dwords_of(long bytes) { return bytes > 0x7ffffffcL ? 0x7ffffffcu
 #if __HIP_DEVICE_COMPILE__
 // 16 bytes per lane from `off` of the resource to LDS, lane by lane from `lds_at` on.  Written out, because
 // the compiler waits for a builtin load of this kind to land before it issues any ds_read_b64_tr_b16, to
-// whatever address; the K loop waits where a buffer changes hands.  (The instruction has no register
-// result; m0 needs one wait state before it.)
+// whatever address; the K loop waits where a buffer changes hands.  The instruction has no register
+// result.  Before it m0 needs one wait state, and a resource register that the vector unit has written (as a
+// readlane does where scalar registers are short) five, which the compiler does not see to in front of
+// written-out code.
 PT_DEV void load_to_lds(v4u rsrc, unsigned lds_at, unsigned off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_at), "v"(off), "s"(rsrc) : "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_at), "v"(off), "s"(rsrc) : "m0");
 }
 // Waits until at most n of this wave's loads are outstanding (vmcnt is split over bits 3:0 and 15:14).
 #define wait_loads(n) __builtin_amdgcn_s_waitcnt(0x0f70 | ((n) & 0xf) | (((n) >> 4) << 14))
