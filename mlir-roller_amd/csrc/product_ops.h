@@ -218,7 +218,8 @@ __global__ __launch_bounds__(256) void zero_kernel(T* c, int ld, int rows, int c
 //
 // SPLIT: x is fp32 although the weights have 16 bits.  Each of its elements then goes into the product as
 // the sum of two of 16 bits, high part and remainder: twice the matrix instructions, which are idle anyway,
-// and no rounding of x that the result could show.
+// and no rounding of x that the result could show.  What the type cannot hold becomes an infinity, as by rounding,
+// without a remainder (infinity less infinity would make it a NaN).
 template <class T, int SPLIT>
 struct x_type { typedef T type; };
 template <class T>
@@ -231,7 +232,8 @@ PT_DEV void split_chunk(const float* x, v4u& hi, v4u& lo) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     h[e] = (T)x[e];
-    l[e] = (T)(x[e] - (float)h[e]);
+    const float rest = x[e] - (float)h[e];
+    l[e] = (T)(fabsf(rest) <= fabsf(x[e]) ? rest : 0.0f);
   }
   hi = __builtin_bit_cast(v4u, h);
   lo = __builtin_bit_cast(v4u, l);

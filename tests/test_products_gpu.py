@@ -290,6 +290,21 @@ def test_gates_far_out(device):
             assert np.linalg.norm(got - want[n][0]) <= 3000 * 2.0 ** -23 * (D + 8) * np.linalg.norm(want[n][0])
 
 
+@pytest.mark.parametrize("T", [1, 3, 7, 16, 20, 80])
+def test_gated_products_beyond_fp16(device, T):
+    # one gated product of 300 * 300 and nothing else: an infinity in fp16, and so is what the weights make of it
+    b = Block(T, 64, 64, "fp16", "silu")
+    for m, value in ((b.x, 1.0), (b.wg, 300.0), (b.wu, 300.0)):
+        m.inside(m.host)[:] = 0
+        m.inside(m.host)[:T if m is b.x else 1, 0] = value
+        m.buffer.set(m.host)
+    b.wd.inside(b.wd.host)[:, 1:] = 0                             # (column 0 belongs to that product)
+    b.wd.buffer.set(b.wd.host)
+    b.forward()
+    hip.synchronize()
+    assert np.array_equal(b.y.get(), np.tile(np.sign(b.wd.inside(b.wd.host)[:, 0].astype(np.float64)) * np.inf, (T, 1)))
+
+
 def test_operands_beyond_4_gib(device):
     # rows so far apart that the last ones lie beyond 2^32 bytes (and 2^31 elements) from the first
     T, D, F, ld = 2304, 64, 96, 1 << 20
