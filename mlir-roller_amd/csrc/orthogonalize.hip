@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long str
     if (t < w) total[t] += total[t + w];
     __syncthreads();
   }
-  const float norm = (float)sqrt(total[0]) + eps;
+  const double inv = 1.0 / (sqrt(total[0]) + (double)eps);   // (a norm beyond fp32 is no infinity here)
   const T* g = G + blockIdx.z * stride;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
   if (tall) {
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void first_kernel(const T* G, int ld, long str
   for (int i = t / 64; i < 64; i += 4) {
     const int r = r0 + i, c = c0 + t % 64;
     float v = tall ? patch[i][t % 64] : c < l && r < s ? (float)g[(long)r * ld + c] : 0.0f;
-    v = v / norm;
+    v = (float)((double)v * inv);
     const long at = blockIdx.z * x_stride + (long)r * pitch + c;
     X[at] = v;
     const Op hi = (Op)(v * kScale);

@@ -420,6 +420,16 @@ def test_orthogonalise_zero_huge_tiny_and_nan(device, dtype):
     assert np.isnan(got[3]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_orthogonalise_a_norm_beyond_fp32(device, dtype):
+    rng = np.random.default_rng(29)
+    base = gradient(rng, 1, 70, 90)[0]
+    G = base * (3e38 / np.abs(base).max())                     # entries up to 3e38, a norm of some 2e39
+    got, G = ortho(G[None], dtype)
+    want = po.orthogonalise(G[0])
+    assert np.linalg.norm(got[0] - want) <= po.orthogonalise_tolerance(G[0], dtype, want)
+
+
 def test_orthogonalise_same_bits(device):
     rng = np.random.default_rng(31)
     G = gradient(rng, 2, 200, 300)
