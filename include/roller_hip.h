@@ -277,9 +277,11 @@ int rl_gemm_f32(const rl_gemm_config* cfg, const float* A, const float* B, float
  *
  * Workspace: the caller's (256-byte aligned, at least what the *_workspace_bytes function says; contents
  * do not matter before or after; calls that share one must not overlap on the device), or NULL for one
- * that the library keeps per stream (grown on demand, which waits for the stream; freed by
- * rl_stream_destroy).  A call on a stream under capture needs the caller's: two graphs that may run at
- * once need one each.  Inputs and outputs must not overlap, unless said otherwise. */
+ * that the library keeps per stream handle (grown on demand, which waits for the stream; freed by
+ * rl_stream_destroy: a stream destroyed in another way leaves it behind, and the next stream that gets
+ * the same handle takes it over, so its work has to be waited for first).  A call on a stream under capture
+ * needs the caller's: two graphs that may run at once need one each.  So does a call on
+ * hipStreamPerThread, which is another stream in every thread.  Inputs and outputs must not overlap, unless said otherwise. */
 
 #define RL_F32 0
 #define RL_F16 1

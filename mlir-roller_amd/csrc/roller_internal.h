@@ -46,7 +46,8 @@ class DeviceScope {
 
 // Workspace of one product call: the caller's, or the library's for the stream (one per stream, grown on
 // demand, held locked until the call has enqueued everything).  The library's is refused while the stream
-// is being captured: the graph would keep an address that a later call may free or share.
+// is being captured (the graph would keep an address that a later call may free or share) and for
+// hipStreamPerThread (one handle, another stream in every thread).
 class ProductRoom {
  public:
   // Takes `need` bytes (rounded up to 256 by the caller); *out may be NULL when need is 0.

@@ -105,6 +105,9 @@ int ProductRoom::take(hipStream_t stream, void* user, size_t user_bytes, size_t 
     return RL_OK;
   }
   if (need == 0) return RL_OK;
+  // (one handle that means another stream in every thread: two of them would work in one buffer at once)
+  if (stream == hipStreamPerThread)
+    return rl_fail(RL_ERR_INVALID_ARG, "%s: a call on the per-thread stream needs the caller's workspace (%zu bytes): the library keeps one per stream handle, and this handle is another stream in every thread", what, need);
   hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
   hipError_t e = hipStreamIsCapturing(stream, &capturing);
   if (e != hipSuccess) return rl_hip_fail(e, "hipStreamIsCapturing");
