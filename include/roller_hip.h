@@ -226,7 +226,8 @@ int rl_gemm_plan_launch(const rl_gemm_plan* plan, const float* A, const float* B
  * before a launch; the kernel leaves them at zero; the area is 256 KiB for up to 65536 tiles and
  * grows beyond) followed by two slots of bm*bn floats per workgroup.  rl_gemm_plan_launch takes it from the library, which keeps one per stream (allocated or
  * grown on first need, which synchronises that stream; launches on one stream run in order, and
- * launches on different streams use different workspaces).  rl_gemm_plan_launch_ws takes it from the
+ * launches on different streams use different workspaces; hipStreamPerThread, one handle for a stream of every
+ * thread, has one for the first thread that uses it, and other threads are refused).  rl_gemm_plan_launch_ws takes it from the
  * caller: `workspace` is device memory, 256-byte aligned, of at least rl_gemm_plan_workspace_bytes
  * bytes, whose first *counter_bytes bytes were zero before its first use -- and are zeroed again by
  * the caller before a launch whose *counter_bytes is larger than that of the launches the workspace

@@ -480,9 +480,24 @@ struct Workspace {
 };
 std::map<hipStream_t, Workspace> g_workspaces;
 std::mutex g_workspaces_mutex;   // (its own lock: launches hold the plan table's shared lock when they get here)
+unsigned long g_per_thread_owner = 0;   // the thread whose hipStreamPerThread has a workspace (thread_number), 0: none
+
+// A number of the calling thread's own, from 1, that no other thread gets.
+unsigned long thread_number() {
+  static std::atomic<unsigned long> last{0};
+  thread_local const unsigned long mine = ++last;
+  return mine;
+}
 
 int workspace_for(hipStream_t stream, size_t bytes, size_t counter_bytes, void** out) {
   std::lock_guard<std::mutex> lock(g_workspaces_mutex);
+  // hipStreamPerThread is one handle and another stream in every thread: its workspace belongs to the first
+  // thread that asks, and a second one, whose launches would run beside the first's, is turned away
+  if (stream == hipStreamPerThread) {
+    if (g_per_thread_owner && g_per_thread_owner != thread_number())
+      return fail(RL_ERR_INVALID_ARG, "stream-K launch on the per-thread stream: the library's workspace for it serves another thread's stream (rl_gemm_plan_launch_ws takes the caller's, of %zu bytes)", bytes);
+    g_per_thread_owner = thread_number();
+  }
   Workspace& w = g_workspaces[stream];
   if (w.bytes >= bytes && w.counter_bytes != counter_bytes) {
     // the counter area moves its end (only launches of more than 65536 tiles differ): what lies between
