@@ -312,7 +312,8 @@ int rl_ffn_workspace_bytes(const rl_ffn_config* cfg, int T, int backward, int un
  * in dtype. */
 int rl_ffn_saved_bytes(const rl_ffn_config* cfg, int T, size_t* bytes);
 
-/* `saved` (256-byte aligned, rl_ffn_saved_bytes) may be NULL: nothing is kept.  T == 0 is a no-op. */
+/* `saved` (256-byte aligned) may be NULL: nothing is kept.  Like the matrices it comes without a size: it holds
+ * rl_ffn_saved_bytes of this T, all of which is written here and read by rl_ffn_backward.  T == 0 is a no-op. */
 int rl_ffn_forward(const rl_ffn_config* cfg, const void* x, int ldx, const void* w_gate, int ld_gate, const void* w_up,
                    int ld_up, const void* w_down, int ld_down, void* y, int ldy, int T, void* saved, void* workspace,
                    size_t workspace_bytes, rl_stream stream);

@@ -18,7 +18,7 @@ import ctypes as C
 from typing import Optional, Sequence
 
 from . import hip
-from .hip import FfnConfig, OrthoConfig, ProductTile, Ptr, _stream_handle, check, lib
+from .hip import RL_ERR_INVALID_ARG, FfnConfig, HipError, OrthoConfig, ProductTile, Ptr, _stream_handle, check, lib
 
 DTYPES = {"fp32": 0, "fp16": 1, "bf16": 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
@@ -68,6 +68,14 @@ class GatedFfn:
         check(lib().rl_ffn_saved_bytes(self._at, tokens, C.byref(out)))
         return out.value
 
+    def _saved(self, saved, nbytes: Optional[int], tokens: int) -> int:
+        """Address of ``saved``, whose size, where it is known, has to hold ``tokens`` (the library is told none)."""
+        if nbytes is None:
+            nbytes = getattr(saved, "nbytes", None)
+        if nbytes is not None and nbytes < self.saved_bytes(tokens):
+            raise HipError(RL_ERR_INVALID_ARG, f"saved: {tokens} tokens need a buffer of {self.saved_bytes(tokens)} bytes, got {nbytes}")
+        return _address(saved)
+
     PRODUCTS = ("gate and up", "down", "dw_down", "dh", "dx", "dw_gate and dw_up")
 
     def tiles(self, tokens: int, compute_units: int = 256) -> dict:
@@ -79,22 +87,25 @@ class GatedFfn:
 
     def forward(self, x, w_gate, w_up, w_down, y, tokens: int, *, ldx: Optional[int] = None, ld_gate: Optional[int] = None,
                 ld_up: Optional[int] = None, ld_down: Optional[int] = None, ldy: Optional[int] = None, saved=None,
-                stream=None, workspace=None, workspace_bytes: Optional[int] = None) -> None:
-        """Enqueues the block for ``tokens`` rows.  ``saved`` (``saved_bytes``) keeps what ``backward`` reads."""
+                stream=None, workspace=None, workspace_bytes: Optional[int] = None, saved_bytes: Optional[int] = None) -> None:
+        """Enqueues the block for ``tokens`` rows.  ``saved`` keeps what ``backward`` reads and has the size that the
+        method ``saved_bytes`` tells: a ``DeviceArray`` is held to it, an address with the argument ``saved_bytes``."""
+        at_saved = None if saved is None else self._saved(saved, saved_bytes, tokens)
         hip.init()
         d, f, room = self.d_model, self.d_ff, _room(workspace, workspace_bytes)
         check(lib().rl_ffn_forward(
             self._at, _address(x), d if ldx is None else ldx, _address(w_gate), d if ld_gate is None else ld_gate,
             _address(w_up), d if ld_up is None else ld_up, _address(w_down), f if ld_down is None else ld_down,
-            _address(y), d if ldy is None else ldy, tokens, None if saved is None else _address(saved), *room, _stream_handle(stream)))
+            _address(y), d if ldy is None else ldy, tokens, at_saved, *room, _stream_handle(stream)))
 
     def backward(self, dy, x, w_gate, w_up, w_down, saved, dx, dw_gate, dw_up, dw_down, tokens: int, *,
                  lddy: Optional[int] = None, ldx: Optional[int] = None, ld_gate: Optional[int] = None, ld_up: Optional[int] = None,
                  ld_down: Optional[int] = None, lddx: Optional[int] = None, ldd_gate: Optional[int] = None,
                  ldd_up: Optional[int] = None, ldd_down: Optional[int] = None, stream=None, workspace=None,
-                 workspace_bytes: Optional[int] = None) -> None:
+                 workspace_bytes: Optional[int] = None, saved_bytes: Optional[int] = None) -> None:
         """Enqueues the gradients of ``sum(dy * y)``.  ``dx``, ``dw_down``, and ``dw_gate`` with ``dw_up``, may be
-        None: not computed."""
+        None: not computed.  ``saved`` as in ``forward``, for as many tokens."""
+        at_saved = self._saved(saved, saved_bytes, tokens)
         hip.init()
         d, f, room = self.d_model, self.d_ff, _room(workspace, workspace_bytes)
         out = [None if g is None else _address(g) for g in (dx, dw_gate, dw_up, dw_down)]

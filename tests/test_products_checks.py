@@ -1,0 +1,29 @@
+"""What the products of a feed-forward block refuse before a device is touched, beside test_products.py."""
+
+import pytest
+
+from mlir_roller_amd import hip
+from mlir_roller_amd.hip import HipError, Ptr
+from mlir_roller_amd.products import GatedFfn
+
+
+class Buffer:
+    """Stands for a device array: an address and a size."""
+
+    def __init__(self, nbytes):
+        self.nbytes = nbytes
+
+    def __int__(self):
+        return 1 << 40
+
+
+def test_a_saved_buffer_for_fewer_tokens_is_refused(hip_lib):
+    op, at = GatedFfn(64, 512, "bf16"), Ptr(1 << 40)
+    need = op.saved_bytes(8)
+    for saved, how in ((Buffer(need - 1), {}), (Buffer(op.saved_bytes(7)), {}), (at, dict(saved_bytes=need - 1)), (Buffer(need), dict(saved_bytes=0))):
+        for call in (lambda: op.forward(at, at, at, at, at, 8, saved=saved, **how),
+                     lambda: op.backward(at, at, at, at, at, saved, at, at, at, at, 8, **how)):
+            with pytest.raises(HipError, match=f"8 tokens need a buffer of {need} bytes") as err:
+                call()
+            assert err.value.status == hip.RL_ERR_INVALID_ARG
+    assert op._saved(Buffer(need), None, 8) == op._saved(at, None, 8) == op._saved(at, need, 8) == 1 << 40
