@@ -54,11 +54,12 @@ PT_DEV float act(float g) {
   return g * sigmoid(GELU_2C * (g + GELU_C1 * g * g * g));   // (1 + tanh z) / 2 = sigmoid(2 z)
 }
 
-// The activation and its slope.  The factors that grow with g stand beside ones that have long been zero
-// where they would overflow, so they are taken of g cut to +-32.
+// The activation and its slope.  The factors that grow with g stand beside ones that are zero in fp32 where they
+// would overflow (the sigmoid from -104 down, earlier the density of gelu and the sigmoid of gelu_tanh), so they are
+// taken of g cut to +-128.
 template <int KIND>
 PT_DEV void act_slope(float g, float& a, float& slope) {
-  const float c = fminf(fmaxf(g, -32.0f), 32.0f);
+  const float c = fminf(fmaxf(g, -128.0f), 128.0f);
   if constexpr (KIND == ACT_SILU) {
     const float s = sigmoid(g);
     a = g * s;

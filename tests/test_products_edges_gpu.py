@@ -1,5 +1,7 @@
-"""The products of a feed-forward block on an MI355X where their other tests do not look: the per-thread stream."""
+"""The products of a feed-forward block on an MI355X where their other tests do not look: activations and slopes far
+below zero, element by element; the per-thread stream."""
 
+import math
 import threading
 
 import numpy as np
@@ -7,9 +9,66 @@ import pytest
 
 from mlir_roller_amd import hip
 from mlir_roller_amd.hip import HipError
+from oracle import products_oracle as po
 from test_products_gpu import Block, room
 
 pytestmark = pytest.mark.gpu
+HALF = 2.0 ** -24                                  # half a step of fp32, relative
+
+
+def fill(m, values):
+    """Other values for a matrix that is on the device."""
+    m.inside(m.host)[:] = po.encode(values, m.dtype)
+    m.values = po.decode(m.inside(m.host), m.dtype)
+    m.buffer.set(m.host)
+
+
+def activation_and_slope(kind, g):
+    """act(g) and act'(g) in 64 bits without the cancellation of 1 + erf and 1 + tanh below zero."""
+    if kind == "gelu":
+        phi = 0.5 * np.vectorize(math.erfc, otypes=[float])(-g / math.sqrt(2))
+        return g * phi, phi + g * np.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    z, dz = (g, 1.0) if kind == "silu" else (math.sqrt(8 / math.pi) * (g + 0.044715 * g ** 3), math.sqrt(8 / math.pi) * (1 + 0.134145 * g * g))
+    s = np.exp(z) / (1 + np.exp(z))
+    return g * s, s + g * s * (1 - s) * dz
+
+
+def gates_alone(device, kind, g):
+    """act(g) and act'(g) as the block computes them in fp32: one token of one feature, up and down weights of one.
+    Every product then is one number times one, and dw_up is the activation and dw_gate the slope."""
+    b = Block(1, 1, len(g), "fp32", kind)
+    for m, v in ((b.x, 1.0), (b.dy, 1.0), (b.wu, 1.0), (b.wd, 1.0), (b.wg, g[:, None])):
+        fill(m, np.broadcast_to(v, (m.rows, m.cols)))
+    saved = room(b.op.saved_bytes(1))
+    b.forward(saved)
+    b.backward(saved)
+    hip.synchronize()
+    return b.wg.values[:, 0], b.grads["dw_up"].get()[:, 0], b.grads["dw_gate"].get()[:, 0]
+
+
+# Relative errors, in half steps.  The exponential's argument carries two half steps of itself (the constant and the
+# product), and so the result 2 |z|; the exponential, the reciprocal, the sum before it and what follows are ten more.
+# z of gelu_tanh has seven half steps of its own (9 |z| in all), and its slope's factor six.  Slope and activation are taken where they are sums
+# of terms of one sign or nearly: beyond -8 (silu) and -3 (gelu_tanh) nothing cancels.  Down to the smallest normal number.
+FAR = [("silu", -8.0, -83.0, lambda g, z: 2 * z + 16), ("gelu_tanh", -3.0, -9.0, lambda g, z: 9 * z + 32)]
+
+
+@pytest.mark.parametrize("kind,near,far,half_steps", FAR)
+def test_activation_and_slope_far_below_zero(device, kind, near, far, half_steps):
+    g, act, slope = gates_alone(device, kind, np.linspace(far, near, 1023))
+    z = np.abs(g) if kind != "gelu_tanh" else math.sqrt(8 / math.pi) * np.abs(g + 0.044715 * g ** 3)
+    want, want_slope = activation_and_slope(kind, g)
+    allowed = half_steps(g, z) * HALF
+    assert (np.abs(slope / want_slope - 1) <= allowed).all(), f"slope off by {np.max(np.abs(slope / want_slope - 1))}"
+    assert (np.abs(act / want - 1) <= allowed).all(), f"activation off by {np.max(np.abs(act / want - 1))}"
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu", "gelu_tanh"])
+def test_ends_of_activation_and_slope(device, kind):
+    g, act, slope = gates_alone(device, kind, np.array([-3e38, -1e30, -1e4, -200.0, -129.0, 0.0, 129.0, 200.0, 1e4, 1e30, 3e38]))
+    assert np.array_equal(act, np.maximum(g, 0)) and np.array_equal(slope, np.where(g < 0, 0, np.where(g == 0, 0.5, 1)))
+
+
 PER_THREAD = 2                                     # hipStreamPerThread: one handle, another stream in every thread
 
 
