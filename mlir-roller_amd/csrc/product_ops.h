@@ -47,10 +47,14 @@ PT_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_am
 
 constexpr float GELU_2C = 1.5957691216f, GELU_C1 = 0.044715f;   // 2 sqrt(2 / pi)
 
+// (1 + erf(g / sqrt 2)) / 2, as erfc of the other sign: 1 + erf has no digits left far below zero (of the activation at -5
+// 3 % were missing, at -6 all of it).
+PT_DEV float normal_below(float g) { return 0.5f * erfcf(-0.70710678f * g); }
+
 template <int KIND>
 PT_DEV float act(float g) {
   if constexpr (KIND == ACT_SILU) return g * sigmoid(g);
-  if constexpr (KIND == ACT_GELU) return 0.5f * g * (1.0f + erff(0.70710678f * g));
+  if constexpr (KIND == ACT_GELU) return g * normal_below(g);
   return g * sigmoid(GELU_2C * (g + GELU_C1 * g * g * g));   // (1 + tanh z) / 2 = sigmoid(2 z)
 }
 
@@ -65,7 +69,7 @@ PT_DEV void act_slope(float g, float& a, float& slope) {
     a = g * s;
     slope = s * (1.0f + c * (1.0f - s));
   } else if constexpr (KIND == ACT_GELU) {
-    const float s = 0.5f * (1.0f + erff(0.70710678f * g));
+    const float s = normal_below(g);
     a = g * s;
     slope = s + c * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * c * c);
   } else {

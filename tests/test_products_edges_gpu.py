@@ -48,9 +48,12 @@ def gates_alone(device, kind, g):
 
 # Relative errors, in half steps.  The exponential's argument carries two half steps of itself (the constant and the
 # product), and so the result 2 |z|; the exponential, the reciprocal, the sum before it and what follows are ten more.
-# z of gelu_tanh has seven half steps of its own (9 |z| in all), and its slope's factor six.  Slope and activation are taken where they are sums
-# of terms of one sign or nearly: beyond -8 (silu) and -3 (gelu_tanh) nothing cancels.  Down to the smallest normal number.
-FAR = [("silu", -8.0, -83.0, lambda g, z: 2 * z + 16), ("gelu_tanh", -3.0, -9.0, lambda g, z: 9 * z + 32)]
+# z of gelu_tanh has seven half steps of its own (9 |z| in all), and its slope's factor six.  gelu: the argument of erfc
+# has two half steps, which move it by 2 g^2 (its logarithm's slope is twice the argument), and the normal density's
+# exponent three, which is 1.5 g^2; erfc itself is right to 16 steps.  Slope and activation are taken where they are sums
+# of terms of one sign or nearly: beyond -8 (silu) and -3 (gelu) nothing cancels.  Down to the smallest normal number.
+FAR = [("silu", -8.0, -83.0, lambda g, z: 2 * z + 16), ("gelu", -3.0, -12.4, lambda g, z: 4 * g * g + 64),
+       ("gelu_tanh", -3.0, -9.0, lambda g, z: 9 * z + 32)]
 
 
 @pytest.mark.parametrize("kind,near,far,half_steps", FAR)
