@@ -7,8 +7,9 @@
 // Two products forward (gate and up share their operand x and come out of one kernel, which also makes h)
 // and four backward (dh with dg and du made on the accumulators; dx as one sum over both pairs; dWg and dWu
 // as the two batch entries of one launch; dWd).  h, dg and du are rounded once to the element type, since
-// the next product's matrix instructions read that type; everything else between the inputs and the outputs
-// is fp32, g and u included, which the forward pass keeps for the backward pass.
+// the next product's matrix instructions read that type (in fp16 dg and du times a power of two, product_ops.h);
+// everything else between the inputs and the outputs is fp32, g and u included, which the forward pass keeps for the
+// backward pass.
 //
 // With up to 16 tokens the forward pass does little but read the weights; it takes few_rows_kernel instead of
 // the tile engine, and with 16-bit types h stays in fp32 there (the second product splits it in two).
@@ -215,6 +216,7 @@ int forward(const FfnCall& c) {
 
 struct BackwardRoom {
   T *dy, *x, *w_gate, *w_up, *w_down, *dg, *du;
+  unsigned* peaks;   // of dy, fp16
   char *arrivals, *pieces;
   Plan dw_down, dh, dx, dw;   // (dw: gate and up)
   size_t bytes;
@@ -235,6 +237,7 @@ BackwardRoom backward_carve(const FfnCall& c, bool unaligned) {
   r.w_gate = pack_space(room, c.F, c.D, weights);
   r.w_up = pack_space(room, c.F, c.D, weights);
   r.w_down = pack_space(room, c.D, c.F, unaligned || !aligned(c.w_down));
+  if (is_scaled<T>()) r.peaks = (unsigned*)room.take(PEAKS * sizeof(unsigned));
   r.arrivals = room.take(kArrivalBytes);
   r.dw_down = plan_dw_down(c);
   r.dh = plan_dh(c);
@@ -260,6 +263,7 @@ int gated_backward(const FfnCall& c, const BackwardRoom& r, const FfnSaved& s, c
   gated.dg = r.dg;
   gated.du = r.du;
   gated.pitch = s.pitch;
+  gated.peaks = r.peaks;
   return run_product<T, 1, 0, 0, 1, 0>(dh, r.dh, gated, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dh");
 }
 
@@ -274,7 +278,15 @@ int backward(const FfnCall& call) {
   const BackwardRoom r = backward_carve(c, false);
   const FfnSaved s = ffn_saved(ES, c.T, c.F);
   const T* h = (const T*)((char*)c.saved + s.h);
-  Arrivals arrivals = arrivals_at(r.arrivals, false);
+  const bool scaled = is_scaled<T>() && (c.dx || c.dw_gate);
+  Arrivals arrivals = arrivals_at(r.arrivals, scaled);   // (cleared by peak_kernel)
+  if constexpr (is_scaled<T>()) {
+    if (scaled) {
+      int lanes = 1;   // per row of dy, 16 bytes each
+      while (lanes < 64 && lanes * PER < c.D) lanes *= 2;
+      PT_TRY(launch<peak_kernel<T>>("ffn: largest gradient", dim3(PEAKS), 256, c.stream, (const T*)c.dy.p, c.dy.ld, c.T, c.D, lanes, r.peaks, arrivals.set[0], kMaxArrivals));
+    }
+  }
   PT_TRY(pack(c.dy, c.T, c.D, r.dy, c.stream));
   if (c.dw_down) {
     const Problem p = problem(c.dy.p, c.dy.ld, h, s.pitch, c.D, c.F, c.T, c.D, c.F);
@@ -294,7 +306,9 @@ int backward(const FfnCall& call) {
     Problem p = problem(r.dg, s.pitch, c.w_gate.p, c.w_gate.ld, c.T, c.D, c.F, c.T, c.D);
     p.a[1] = r.du;
     p.b[1] = c.w_up.p;
-    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, r.dx, store(c.dx, c.ld_dx, c.D), 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
+    Store<T> out = store(c.dx, c.ld_dx, c.D);
+    out.peaks = r.peaks;
+    PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, r.dx, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
   }
   if (c.dw_gate) {
     PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
@@ -303,6 +317,7 @@ int backward(const FfnCall& call) {
     Store<T> out = store(c.dw_gate, c.ld_dw_gate, c.D);
     out.c[1] = (T*)c.dw_up;
     out.ldc1 = c.ld_dw_up;
+    out.peaks = r.peaks;
     out.vec = out.vec && vec_ok(c.dw_up, c.ld_dw_up);
     PT_TRY((run_product<T, 0, 0, 0, 1, 0>(p, r.dw, out, 2, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dw_gate and dw_up")));
   }

@@ -79,6 +79,36 @@ PT_DEV void act_slope(float g, float& a, float& slope) {
   }
 }
 
+// ---- the scale of fp16 gradients --------------------------------------------------------------------
+// dg and du are operands of two further products and have the element type.  In fp16 a number below 2^-14 has fewer
+// than 11 bits, and that is where the gradients of an unscaled loss are (dy of 1e-6: dW_gate 3 % off).  So they are
+// held times 2^k, and the products made of them leave times 2^-k.  k >= 0 is the least that brings the largest
+// finite |dy| to 2^-6: dg and du around 2^-9 then have all their bits, and they reach infinity at 2^22 times that
+// |dy|.  From |dy| = 2^-6 on k is 0.  (bf16 has the exponents of fp32.)
+
+constexpr int PEAKS = 256;   // workgroups of peak_kernel
+
+template <class T>
+constexpr bool is_scaled() { return __is_same(T, half_t); }
+
+// 2^k (SIGN 1) or 2^-k (SIGN -1) by the peaks of dy, each of which is a fp16 magnitude's bits.  By whole waves.
+template <int SIGN>
+PT_DEV float power_of_peaks(const unsigned* peaks) {
+  const v4u four = *(const v4u*)(peaks + 4 * (threadIdx.x & 63));
+  unsigned peak = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) peak = four[e] > peak ? four[e] : peak;
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    const unsigned other = __shfl_xor(peak, d);
+    peak = other > peak ? other : peak;
+  }
+  const float value = (float)__builtin_bit_cast(half_t, (unsigned short)__builtin_amdgcn_readfirstlane(peak));
+  const int exponent = (int)(__builtin_bit_cast(unsigned, value) >> 23) - 127;
+  const int k = value > 0.0f && exponent < -6 ? -6 - exponent : 0;   // (18 at most)
+  return __builtin_bit_cast(float, (unsigned)(127 + SIGN * k) << 23);
+}
+
 // ---- epilogues --------------------------------------------------------------------------------------
 
 // C = acc, in a caller's matrix: any leading dimension and alignment.
@@ -87,18 +117,22 @@ struct Store {
   T* c[2];      // one per batch entry
   int ldc, ldc1, N;
   int vec;      // rows of 4 elements are aligned
+  const unsigned* peaks;   // fp16: of the dy by which an operand is scaled, NULL: none is
+  float scale;             // (by at)
   __device__ __forceinline__ Store at(int batch) const {
     Store o = *this;
     if (batch) {
       o.c[0] = c[1];
       o.ldc = ldc1;
     }
+    if constexpr (is_scaled<T>()) o.scale = peaks ? power_of_peaks<-1>(peaks) : 1.0f;
     return o;
   }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
   __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const {
     if (!ok) return;
+    if constexpr (is_scaled<T>()) v *= scale;
     T* to = c[0] + (long)m * ldc + n;
     if (vec && n + 3 < N) {
       store4(to, v);
@@ -136,13 +170,19 @@ struct GatedForward {
   }
 };
 
-// From dh: dg = dh u act'(g), du = dh act(g).
+// From dh: dg = dh u act'(g), du = dh act(g), in fp16 times 2^k.
 template <class T, int KIND>
 struct GatedBackward {
   const float *g, *u;
   T *dg, *du;
   int pitch;
-  __device__ __forceinline__ GatedBackward at(int) const { return *this; }
+  const unsigned* peaks;   // fp16: of dy
+  float scale;             // (by at)
+  __device__ __forceinline__ GatedBackward at(int) const {
+    GatedBackward o = *this;
+    if constexpr (is_scaled<T>()) o.scale = power_of_peaks<1>(peaks);
+    return o;
+  }
   struct In {
     v4f gate, up;
   };
@@ -152,6 +192,7 @@ struct GatedBackward {
   }
   __device__ __forceinline__ void put(int m, int n, v4f dh, In in, bool ok) const {
     const long i = (long)m * pitch + n;
+    if constexpr (is_scaled<T>()) dh *= scale;
     v4f x, y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -196,6 +237,41 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int ld, int row
   for (long i = blockIdx.x * 256L + threadIdx.x; i < (long)rows * chunks; i += gridDim.x * 256L) {
     const int r = (int)(i / chunks), c = (int)(i % chunks) * PER;
     *(v4u*)(dst + (long)r * pitch + c) = chunk_at(src + (long)r * ld, c, cols);
+  }
+}
+
+// The largest finite |element| of each of PEAKS shares of a fp16 matrix, as the bits of a magnitude, which are in the order
+// of the numbers; zeros in `clear`.  `lanes` lanes, a power of two, read a row side by side.
+template <class T>
+__global__ __launch_bounds__(256) void peak_kernel(const T* src, int ld, int rows, int cols, int lanes, unsigned* peaks, unsigned* clear, int n_clear) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n_clear; i += gridDim.x * 256) clear[i] = 0;
+  constexpr int PER = 16 / sizeof(T), UNROLL = 4;
+  const int chunks = (cols + PER - 1) / PER, side = 256 / lanes;
+  unsigned peak = 0;
+  for (long r = (long)blockIdx.x * side + threadIdx.x / lanes; r < rows; r += (long)gridDim.x * side)
+    for (int c = threadIdx.x % lanes; c < chunks; c += lanes * UNROLL) {
+      v4u v[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) v[u] = chunk_at(src + r * ld, (c + lanes * u) * PER, cols);   // (zeros past the end)
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const unsigned bits = v[u][e / 2] >> (e % 2 * 16) & 0x7fff;
+          peak = bits < 0x7c00 && bits > peak ? bits : peak;
+        }
+    }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    const unsigned other = __shfl_xor(peak, d);
+    peak = other > peak ? other : peak;
+  }
+  __shared__ unsigned waves[4];
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = peak;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 4; ++w) peak = waves[w] > peak ? waves[w] : peak;
+    peaks[blockIdx.x] = peak;
   }
 }
 

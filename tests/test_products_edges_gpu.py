@@ -1,5 +1,5 @@
 """The products of a feed-forward block on an MI355X where their other tests do not look: activations and slopes far
-below zero, element by element; the per-thread stream."""
+below zero, element by element; fp16 gradients that are subnormal before they are summed; the per-thread stream."""
 
 import math
 import threading
@@ -10,7 +10,7 @@ import pytest
 from mlir_roller_amd import hip
 from mlir_roller_amd.hip import HipError
 from oracle import products_oracle as po
-from test_products_gpu import Block, room
+from test_products_gpu import Block, Graph, room
 
 pytestmark = pytest.mark.gpu
 HALF = 2.0 ** -24                                  # half a step of fp32, relative
@@ -70,6 +70,65 @@ def test_activation_and_slope_far_below_zero(device, kind, near, far, half_steps
 def test_ends_of_activation_and_slope(device, kind):
     g, act, slope = gates_alone(device, kind, np.array([-3e38, -1e30, -1e4, -200.0, -129.0, 0.0, 129.0, 200.0, 1e4, 1e30, 3e38]))
     assert np.array_equal(act, np.maximum(g, 0)) and np.array_equal(slope, np.where(g < 0, 0, np.where(g == 0, 0.5, 1)))
+
+
+# fp16 gradients of the size that an unscaled loss has: dg and du are products of dy, and below 6e-5 a fp16 number has
+# fewer than 11 bits.  The sums over 2048 tokens that they go into are 50 times larger and can be told apart.  Allowed in
+# the norm: 2^-25 an element, the most that rounding a subnormal output takes, and 2^-10 of it, twice what one rounding of every
+# term (2^-11 of each at most, independent of each other) and one of the output come to.
+@pytest.mark.parametrize("rms", [1e-6, 1e-5, 1e-3, 1.0])
+def test_small_gradients_in_fp16(device, rms):
+    b = Block(2048, 64, 96, "fp16", "silu")
+    fill(b.dy, rms * np.random.default_rng(7).standard_normal((2048, 64)))
+    saved = room(b.op.saved_bytes(2048))
+    b.forward(saved)
+    b.backward(saved)
+    hip.synchronize()
+    want = b.want.backward(b.dy.values)
+    for n, g in b.grads.items():
+        value = want[n][0]
+        off = np.linalg.norm(g.get() - value)
+        assert off <= math.sqrt(value.size) * 2.0 ** -25 + 2.0 ** -10 * np.linalg.norm(value), f"{n} off by {off / np.linalg.norm(value)}"
+
+
+def test_small_gradients_beside_a_token_of_nan_and_infinities(device):
+    # what is not finite in dy does not decide how the other tokens' gradients are rounded
+    b = Block(300, 64, 2048, "fp16", "silu")
+    small = 1e-5 * np.random.default_rng(8).standard_normal((300, 64))
+    small[5], small[77, 3], small[200] = np.nan, np.inf, 0.0
+    fill(b.dy, small)
+    saved = room(b.op.saved_bytes(300))
+    b.forward(saved)
+    b.backward(saved, ("dx",))
+    hip.synchronize()
+    keep = [t for t in range(300) if t not in (5, 77)]
+    few = po.FeedForward(b.x.values[keep], b.wg.values, b.wu.values, b.wd.values, "silu", "fp16").backward(b.dy.values[keep])["dx"][0]
+    got = b.grads["dx"].get()
+    assert np.isnan(got[5]).all() and not got[200].any()
+    assert np.linalg.norm(got[keep] - few) <= math.sqrt(few.size) * 2.0 ** -25 + 2.0 ** -10 * np.linalg.norm(few)
+
+
+def test_a_captured_backward_pass_scales_by_the_gradients_of_the_replay(device):
+    b = Block(200, 136, 264, "fp16", "silu")
+    stream, saved, ws = hip.Stream(), room(b.op.saved_bytes(200)), room(b.op.workspace_bytes(200, backward=True))
+    b.forward(saved)
+    hip.synchronize()
+    graph = Graph(stream)
+    with graph:
+        b.backward(saved, workspace=ws, stream=stream)
+    values = np.random.default_rng(9).standard_normal((200, 136))
+    for rms in (1e-6, 1.0, 1e-4, 0.0, 1e-5):
+        fill(b.dy, rms * values)
+        b.backward(saved, workspace=ws, stream=stream)
+        hip.synchronize()
+        eager = [m.bits() for m in b.grads.values()]
+        for m in b.grads.values():
+            m.buffer.fill_bytes(0xFF)
+        ws.fill_bytes(0xFF)
+        hip.synchronize()
+        graph.launch(stream)
+        hip.synchronize()
+        assert all(np.array_equal(p, m.bits()) for p, m in zip(eager, b.grads.values())), f"replay on gradients of {rms}"
 
 
 PER_THREAD = 2                                     # hipStreamPerThread: one handle, another stream in every thread
