@@ -316,7 +316,7 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   }
   const int m0 = tile_m * S::BM, n0 = tile_n * S::OUT_N;
 
-  for (int i = blockIdx.x * NT + tid; i < p.n_clear; i += gridDim.x * NT) p.clear[i] = 0;
+  for (long i = (long)blockIdx.x * NT + tid; i < p.n_clear; i += (long)gridDim.x * NT) p.clear[i] = 0;   // (beyond 2^31 threads)
 
   // K steps of this workgroup.  A segment is a whole number of steps: its last step is cut by K.
   const int seg_steps = (p.K + S::KSTEP - 1) / S::KSTEP;

@@ -1,5 +1,6 @@
 """The products of a feed-forward block on an MI355X where their other tests do not look: activations and slopes far
-below zero, element by element; fp16 gradients that are subnormal before they are summed; the per-thread stream."""
+below zero, element by element; fp16 gradients that are subnormal before they are summed; a launch of more than 2^31
+threads; the per-thread stream."""
 
 import math
 import threading
@@ -8,9 +9,10 @@ import numpy as np
 import pytest
 
 from mlir_roller_amd import hip
-from mlir_roller_amd.hip import HipError
+from mlir_roller_amd.hip import DeviceArray, HipError
+from mlir_roller_amd.products import GatedFfn
 from oracle import products_oracle as po
-from test_products_gpu import Block, Graph, room
+from test_products_gpu import Block, Graph, Matrix, room
 
 pytestmark = pytest.mark.gpu
 HALF = 2.0 ** -24                                  # half a step of fp32, relative
@@ -129,6 +131,29 @@ def test_a_captured_backward_pass_scales_by_the_gradients_of_the_replay(device):
         graph.launch(stream)
         hip.synchronize()
         assert all(np.array_equal(p, m.bits()) for p, m in zip(eager, b.grads.values())), f"replay on gradients of {rms}"
+
+
+def test_more_than_2_to_the_31_threads(device):
+    # 16 million tokens through 64 x 64 tiles: 8.65 million workgroups of 256 threads.  The tokens are one stretch of
+    # 100003 again and again; what is looked at is the ends, a stretch 2^31 elements before the end of h, and others
+    T, D, F, period = 16776704, 283, 1033, 100003
+    op, rng = GatedFfn(D, F, "fp32"), np.random.default_rng(11)
+    rows, cols, splits, whole = op.tiles(T, device.compute_units)["gate and up"]
+    assert (rows, cols, splits) == (64, 64, 1) and whole * 256 > 1 << 31
+    stretch = rng.standard_normal((period, D)).astype(np.float32)
+    weights = [Matrix(s * rng.standard_normal(shape), "fp32") for shape, s in (((F, D), D ** -0.5), ((F, D), D ** -0.5), ((D, F), F ** -0.5))]
+    x, y = DeviceArray((T, D)), DeviceArray((T, D))
+    for t in range(0, T, period):
+        hip.check(hip.lib().rl_memcpy_h2d(int(x.ptr) + t * D * 4, stretch.ctypes.data, min(period, T - t) * D * 4))
+    ws = DeviceArray((op.workspace_bytes(T),), np.uint8)
+    op.forward(x, *[w.ptr for w in weights], y, T, workspace=ws)
+    hip.synchronize()
+    for start in (0, T - 2 ** 31 // 1056 - 4096, T - 2 ** 31 // 1056 + 1000, T - 4096, *rng.integers(0, T - 4096, 4)):
+        got = np.empty((4096, D), np.float32)
+        hip.check(hip.lib().rl_memcpy_d2h(got.ctypes.data, int(y.ptr) + int(start) * D * 4, got.nbytes))
+        want = po.FeedForward(stretch[np.arange(start, start + 4096) % period].astype(np.float64), *[w.values for w in weights], "silu", "fp32")
+        assert (np.abs(got - want.y) <= want.y_bound).all(), f"tokens from {start}"
+    x.free(), y.free(), ws.free()
 
 
 PER_THREAD = 2                                     # hipStreamPerThread: one handle, another stream in every thread
