@@ -69,7 +69,7 @@ int launch_tile(const Problem& p, const Epi& epi, int batch, hipStream_t stream,
   static_assert(t::BM == kTiles[K].bm && t::BN == kTiles[K].bn, "the plan's tiles");
   const long nbm = (p.M_out + S::BM - 1) / S::BM, nbn = (p.N_out + S::OUT_N - 1) / S::OUT_N;
   const long tiles = (SYM ? nbm * (nbm + 1) / 2 : nbm * nbn) * batch, groups = p.whole + (tiles - p.whole) * p.splits;
-  if (groups > 0xffffff) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
+  if (groups > kMaxGroups) return rl_fail(RL_ERR_INVALID_ARG, "%s: %ld workgroups are more than one launch takes", what, groups);
   return launch<tile_kernel<S, Epi>>(what, dim3((unsigned)groups), S::NT, stream, p, epi);
 }
 

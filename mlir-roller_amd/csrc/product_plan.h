@@ -37,6 +37,7 @@ constexpr float kClearLaunch = 3.0f;        // a launch that clears the arrival 
 constexpr int kMaxSplits = 16;
 constexpr int kMaxArrivals = 4096;          // tiles of a split product
 constexpr size_t kMaxPieces = (size_t)1 << 29;
+constexpr long kMaxGroups = 0xffffff;       // workgroups of a launch (below 2^32 threads)
 
 struct Plan {
   float time;   // microseconds, by the model
@@ -67,6 +68,8 @@ inline Plan plan_product(int elem_bytes, int gated, int segs, int sym, int M_out
         if (tail && (splits == 1 || whole == 0 || whole == tiles || compute_units % XCDS != 0)) continue;
         const size_t pieces = (size_t)(tiles - whole) * splits * c.bm * c.bn * 4;
         if (pieces > kMaxPieces || tiles - whole > kMaxArrivals) continue;
+        // (the largest tile stays in any case: what is too much for it is refused)
+        if (t != 0 && whole + (tiles - whole) * splits > kMaxGroups) continue;
         const long alone = (whole + compute_units - 1) / compute_units, shared = ((tiles - whole) * splits + compute_units - 1) / compute_units;
         float time = once + alone * (steps * step + fixed) + shared * (per * step + fixed);
         if (splits > 1) time += kJoinPiece * splits + 2.0f * pieces / kPieceBytes;

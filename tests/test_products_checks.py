@@ -1,4 +1,5 @@
-"""What the products of a feed-forward block refuse before a device is touched, beside test_products.py."""
+"""What the products of a feed-forward block refuse, and what they choose, before a device is touched, beside
+test_products.py."""
 
 import pytest
 
@@ -27,3 +28,12 @@ def test_a_saved_buffer_for_fewer_tokens_is_refused(hip_lib):
                 call()
             assert err.value.status == hip.RL_ERR_INVALID_ARG
     assert op._saved(Buffer(need), None, 8) == op._saved(at, None, 8) == op._saved(at, need, 8) == 1 << 40
+
+
+@pytest.mark.parametrize("T,D,F", [(1 << 24, 5, 2024), (1 << 24, 4, 997), (1 << 24, 1986, 6)])
+def test_many_tokens_of_a_small_block_fit_one_launch(hip_lib, T, D, F):
+    # rows x columns of results in tiles; gate and up columns count both
+    for name, columns in (("gate and up", 2 * F), ("down", D)):
+        rows, cols, splits, whole = GatedFfn(D, F, "fp32").tiles(T)[name]
+        tiles = -(-T // rows) * -(-columns // cols)
+        assert whole + (tiles - whole) * splits <= 0xFFFFFF
