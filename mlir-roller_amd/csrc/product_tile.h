@@ -316,7 +316,8 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   }
   const int m0 = tile_m * S::BM, n0 = tile_n * S::OUT_N;
 
-  for (long i = (long)blockIdx.x * NT + tid; i < p.n_clear; i += (long)gridDim.x * NT) p.clear[i] = 0;   // (beyond 2^31 threads)
+  // (unsigned: there may be almost 2^32 threads; where the step wraps around it goes back by 256 or more, and ends)
+  for (unsigned i = blockIdx.x * NT + tid; i < (unsigned)p.n_clear; i += gridDim.x * NT) p.clear[i] = 0;
 
   // K steps of this workgroup.  A segment is a whole number of steps: its last step is cut by K.
   const int seg_steps = (p.K + S::KSTEP - 1) / S::KSTEP;
@@ -687,14 +688,18 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
   const unsigned mine = wave * (MI * PITCH * 4);
   const unsigned to = mine + (lr * PITCH + 4 * lg) * 4;
   const auto out = epi.at(batch);
+  // (what one lane writes another reads; the LDS serves a wave's accesses in their order, which the compiler has to keep)
+  auto lanes_meet = []() __attribute__((always_inline)) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); };
   {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      lanes_meet();
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int q = 0; q < REGS / 4; ++q)   // registers 4q .. 4q+3: columns 256 / MI * q + 4 * lg and on of the block
           lds_write(to + (j * MI + 256 / MI * q) * 4, v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+      lanes_meet();
       const int mb = m0 + wm0 + i * MI;
       constexpr int COLS = S::GATED ? S::WN / 2 : S::WN, PER_ROW = COLS / 4, UNITS = MI * PER_ROW;   // 4 columns a unit
       const int nb = n0 + (S::GATED ? (wave % S::NWN) * (S::WN / 2) : wn0);
@@ -741,7 +746,10 @@ __global__ __launch_bounds__(S::NT, S::PER_CU * S::WAVES / 4 > 0 ? S::PER_CU * S
       // the mirror image of a tile below the diagonal, of the values that have just left: four rows of one column
       // a unit
       if constexpr (S::SYM) {
-        if (tile_m != tile_n) units(int_c<1>{});
+        if (tile_m != tile_n) {
+          lanes_meet();
+          units(int_c<1>{});
+        }
       }
     }
   }
