@@ -151,3 +151,56 @@ def orthogonalise_tolerance(G: np.ndarray, dtype: str, exact: np.ndarray, **how)
     norm = np.linalg.norm(exact)
     n = max(G.shape)
     return 3 * np.linalg.norm(model - exact) + (64 * sqrt(n) * 2.0 ** -24 + HALF_STEP[dtype]) * norm + SMALLEST[dtype] * sqrt(exact.size)
+
+
+def orthogonalise_two_part(G: np.ndarray, steps: int = 5, coefficients=STANDARD, eps: float = 1e-7, scale: float = 1.0, lose=()) -> np.ndarray:
+    """Newton-Schulz as fp16 and fp32 matrices take it, in fp32 on the host: operands are two fp16 numbers, scaled by 2^9,
+    and a product is hi hi + hi lo + lo hi.  ``lose`` leaves terms out: "hi lo", "lo hi"."""
+    f = np.float32
+    tall = G.shape[0] > G.shape[1]
+    X = G.T if tall else G
+    X = np.ascontiguousarray((X / (np.sqrt((X * X).sum()) + eps)).astype(f))
+
+    def parts(M):
+        M = M * f(512)
+        hi = M.astype(np.float16).astype(f)
+        return hi, (M - hi).astype(np.float16).astype(f)
+
+    def product(a, b):
+        p = a[0] @ b[0]
+        if "hi lo" not in lose:
+            p += a[0] @ b[1]
+        if "lo hi" not in lose:
+            p += a[1] @ b[0]
+        return p * f(2.0 ** -18)
+
+    per_step = coefficients if steps and np.ndim(coefficients) == 2 else [coefficients] * steps
+    for a, b, c in ([f(v) for v in step] for step in per_step):
+        x = parts(X)
+        A = product(x, [np.ascontiguousarray(p.T) for p in x])
+        D = np.diag(A).copy()
+        ao = parts(A - np.diag(D))
+        Ao, square = (ao[0] + ao[1]) * f(1 / 512), product(ao, ao)
+        B = b * Ao + c * (square + (D[:, None] + D[None, :]) * Ao)
+        E = b * D + c * (np.diag(square) + D * D)
+        np.fill_diagonal(B, 0)
+        X = (a + E)[:, None] * X + product(parts(B), x)
+    X = scale * X.astype(np.float64)
+    return X.T if tall else X
+
+
+def two_part_excess(got: np.ndarray, exact: np.ndarray, model: np.ndarray, dtype: str) -> float:
+    """How far fp16 or fp32 results are off, in the norm, as a multiple of what they may be.
+
+    ``model`` (orthogonalise_two_part) has the library's roundings and sums of fp32 in another order, one rounding per
+    product where a matrix unit has one per 16, so its error e stands for the library's; four times it is allowed, and
+    half a step of the output.  For fp16 that half step is 500 times e; the result is held to the exact one after its rounding
+    instead.  The two differ where an error of e_i takes an element over the border between two numbers, a step s_i apart:
+    with probability |e_i| / s_i, which adds s_i^2; so the square of the norm is sum |e_i| s_i, at most |e| |s|, and
+    where e_i is more than a step, |e|^2."""
+    e = 4 * np.linalg.norm(model - exact)
+    if dtype == "fp32":
+        return np.linalg.norm(got - exact) / (e + HALF_STEP[dtype] * np.linalg.norm(exact))
+    rounded = exact.astype(np.float16)
+    steps = np.maximum(np.spacing(np.abs(rounded)).astype(np.float64), 2.0 ** -24)
+    return np.linalg.norm(got - rounded.astype(np.float64)) / (np.sqrt(e * np.linalg.norm(steps)) + e)
