@@ -38,7 +38,11 @@ def _address(x) -> int:
 def _room(workspace, workspace_bytes: Optional[int]) -> tuple[Optional[int], int]:
     if workspace is None:
         return None, 0
-    return _address(workspace), int(workspace.nbytes if workspace_bytes is None else workspace_bytes)
+    if workspace_bytes is None:
+        workspace_bytes = getattr(workspace, "nbytes", None)
+        if workspace_bytes is None:
+            raise ValueError("workspace: an address needs its size as workspace_bytes")
+    return _address(workspace), int(workspace_bytes)
 
 
 class GatedFfn:

@@ -3,7 +3,7 @@ test_products.py."""
 
 import pytest
 
-from mlir_roller_amd import hip
+from mlir_roller_amd import hip, products
 from mlir_roller_amd.hip import HipError, Ptr
 from mlir_roller_amd.products import GatedFfn
 
@@ -28,6 +28,13 @@ def test_a_saved_buffer_for_fewer_tokens_is_refused(hip_lib):
                 call()
             assert err.value.status == hip.RL_ERR_INVALID_ARG
     assert op._saved(Buffer(need), None, 8) == op._saved(at, None, 8) == op._saved(at, need, 8) == 1 << 40
+
+
+def test_the_size_of_a_workspace_is_asked_for():
+    assert products._room(None, None) == (None, 0) and products._room(Buffer(512), None) == (1 << 40, 512) and products._room(Ptr(256), 512) == (256, 512)
+    for address in (Ptr(256), 256):
+        with pytest.raises(ValueError, match="needs its size as workspace_bytes"):
+            products._room(address, None)
 
 
 @pytest.mark.parametrize("T,D,F", [(1 << 24, 5, 2024), (1 << 24, 4, 997), (1 << 24, 1986, 6)])
