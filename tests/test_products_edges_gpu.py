@@ -1,16 +1,19 @@
 """The products of a feed-forward block on an MI355X where their other tests do not look: activations and slopes far
 below zero, element by element; fp16 gradients that are subnormal before they are summed; a launch of more than 2^31
-threads; the per-thread stream."""
+threads; captured first calls; large stacks; the per-thread stream."""
 
 import math
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
 
 from mlir_roller_amd import hip
 from mlir_roller_amd.hip import DeviceArray, HipError
-from mlir_roller_amd.products import GatedFfn
+from mlir_roller_amd.products import GatedFfn, Orthogonalizer
 from oracle import products_oracle as po
 from test_products_gpu import Block, Graph, Matrix, room
 
@@ -154,6 +157,57 @@ def test_more_than_2_to_the_31_threads(device):
         want = po.FeedForward(stretch[np.arange(start, start + 4096) % period].astype(np.float64), *[w.values for w in weights], "silu", "fp32")
         assert (np.abs(got - want.y) <= want.y_bound).all(), f"tokens from {start}"
     x.free(), y.free(), ws.free()
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import numpy as np
+from mlir_roller_amd import hip
+from mlir_roller_amd.products import Orthogonalizer
+from test_products_gpu import Block, Graph, Matrix, gradient, room
+hip.init(0)
+b, stream = Block(200, 136, 264, "fp16", "silu"), hip.Stream()
+saved, ws = room(b.op.saved_bytes(200)), room(b.op.workspace_bytes(200, backward=True))
+G, O = Matrix(gradient(np.random.default_rng(1), 1, 60, 90)[0], "fp16"), Matrix(None, "fp16", shape=(60, 90))
+o = Orthogonalizer(60, 90, dtype="fp16")
+ws_o, graph = room(o.workspace_bytes()), Graph(stream)
+with graph:
+    b.forward(saved, workspace=ws, stream=stream)
+    b.backward(saved, workspace=ws, stream=stream)
+    o.launch(G.ptr, O.ptr, workspace=ws_o, stream=stream)
+for _ in range(3):
+    graph.launch(stream)
+b.check_y()
+b.check_grads()
+captured = O.bits()
+o.launch(G.ptr, O.ptr, workspace=ws_o, stream=stream)
+hip.synchronize()
+assert np.array_equal(captured, O.bits())
+print("captured and right")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(device):
+    tests = Path(__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL, str(tests), str(tests.parent)], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "captured and right" in done.stdout, done.stderr
+
+
+# ends of the documented ranges
+@pytest.mark.parametrize("rows,cols,dtype", [(8, 5, "fp32"), (3, 9, "bf16")])
+def test_a_stack_of_65535_matrices(device, rows, cols, dtype):
+    few = po.encode(1e-3 * np.random.default_rng(1).standard_normal((50, rows, cols)), dtype)
+    G = DeviceArray.from_host(few[np.arange(65535) % 50])
+    op = Orthogonalizer(rows, cols, batch=65535, dtype=dtype)
+    ws = DeviceArray((op.workspace_bytes(),), np.uint8)
+    op.launch(G, G, workspace=ws)
+    hip.synchronize()
+    got = po.decode(G.get(), dtype)
+    for i in range(50):
+        value = po.decode(few[i], dtype)
+        want = po.orthogonalise(value)
+        assert np.max(np.linalg.norm(got[i::50] - want, axis=(1, 2))) <= po.orthogonalise_tolerance(value, dtype, want)
 
 
 PER_THREAD = 2                                     # hipStreamPerThread: one handle, another stream in every thread

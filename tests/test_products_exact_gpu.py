@@ -75,3 +75,10 @@ def test_more_tokens_at_odd_rows(device, T, D, F, dtype):
     b = ExactFeedForward(T, D, F, dtype)
     compare(b, run(b))
     compare(b, run(b, 2, 1, backward=False))
+
+
+# ends of the documented ranges
+@pytest.mark.parametrize("T,D,F,dtype", [(3, 1 << 20, 2, "bf16"), (3, 2, 1 << 20, "fp32"), (40, 1 << 20, 3, "fp16"), (200, 7, (1 << 20) - 1, "bf16"), (1 << 20, 1, 1, "bf16")])
+def test_long_rows_and_many_tokens(device, T, D, F, dtype):
+    b = ExactFeedForward(T, D, F, dtype)
+    compare(b, run(b), np.arange(T)[::-(-T // 300)], np.arange(F)[::-(-F // 300)])
