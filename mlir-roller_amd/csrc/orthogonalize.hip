@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) void transposed_out_kernel(const float* X, int
     if (c0 + i < l && r0 + t % 64 < s) O[blockIdx.z * stride + (long)(c0 + i) * ldo + r0 + t % 64] = (T)(patch[t % 64][i] * scale);
 }
 
-// O = scale X without a step (steps = 0), and for a wide matrix whose last step ran elsewhere.
+// O = scale X without a step (steps = 0) for a matrix that is not tall; with steps the last one writes O.
 template <class T>
 __global__ __launch_bounds__(256) void out_kernel(const float* X, int s, int l, int pitch, long x_stride, float scale, T* O, int ldo, long stride) {
   const float* x = X + blockIdx.z * x_stride;

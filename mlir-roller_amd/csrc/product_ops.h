@@ -377,7 +377,7 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(const typename x_type<T,
       }
   }
 
-  // the waves' sums, added in wave order, and the parts' in part order, by wave b for block b
+  // the waves' sums, added in wave order, and the parts' in part order, block after block by the first wave
   __shared__ v4f sums[W][16][64];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {

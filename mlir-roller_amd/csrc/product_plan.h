@@ -8,10 +8,16 @@
 namespace product {
 
 // What a tile costs on one compute unit, in microseconds: `step` per K step of 128 bytes, `fixed` for first
-// loads and epilogue, `once` for the launch.  Fitted to 3588 timed products (32 to 8192 rows, 64 to 11000
-// columns, K 64 to 11000, operands out of memory; K-major and row-major operands; whole tiles, all split, the
-// last round split): the model is off by 13 % (16 bits) and 7 % (32 bits) rms, and what it chooses is on average
-// 1 %, at worst 19 %, slower than the fastest choice timed.
+// loads and epilogue, `once` for the launch.  Fitted to 3588 timings of 339 products that store their sums and
+// nothing else (32 to 8192 rows, 64 to 11000 columns, K 64 to 11000, three sets of operands in turn, most of which
+// the 256 MB cache before the memory holds; K-major and row-major operands; whole tiles, all split, the last round
+// split; some ms of work at a time): there it is off by 13 % (16 bits) and 7 % (32 bits) rms, and what it chooses is on
+// average 1 %, at worst 19 %, slower than the fastest choice timed.
+// It ranks tiles of one product and does not foretell times.  It has no term for the memory, for what an epilogue
+// reads and writes besides the result, or for the clock that the card keeps under a long load, which are much the same
+// for every tile; products that are bound by those take up to 2.8 times as long as it says (24 tokens, gate and up weights
+// of 134 MB: 12.6 us by the model, 25 of the memory; 4096 x 4096 update, B X with X in fp32: 70 and 134).  Rounds are
+// counted by CUs also for the tiles of which a CU holds two or three.
 // The large tiles have the higher rate where they fill the CUs (4096^3 in bf16: 103 us with 256 x 256 tiles,
 // 113 with 192, 120 with 128, 191 with 64); the small ones where the others would not (1024 x 1920 x 5000:
 // 118, 65, 49 and 46 us unsplit), and 192 x 192 makes the lower triangle of 4096 x 4096 253 tiles for 256 CUs.

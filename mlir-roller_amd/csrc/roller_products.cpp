@@ -44,7 +44,7 @@ int check_matrix(const char* name, const void* p, int ld, int cols, int es) {
   return RL_OK;
 }
 
-// (the widest row that check_matrix lets through, for extents)
+// Extents: their dense rows, and the internal ones that are up to two lines longer, are within what check_matrix lets through.
 constexpr int kMaxExtent = (1 << 20);
 
 int check_stream(hipStream_t stream, int device) {

@@ -126,7 +126,8 @@ class Orthogonalizer:
     ``X = G / (||G|| + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` of the
     shorter side, and ``O = scale X``.
 
-    ``coefficients`` is one ``(a, b, c)`` for all steps, or one for each."""
+    ``coefficients`` is one ``(a, b, c)`` for all steps, or one for each; they keep the elements of X, A and
+    b A + c A A below 100."""
 
     STANDARD = (3.4445, -4.7750, 2.0315)
 
