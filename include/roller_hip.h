@@ -359,7 +359,7 @@ int rl_ortho_tiles(const rl_ortho_config* cfg, int compute_units, rl_product_til
 /* `coefficients`: host memory, (a, b, c) for each step, read before the call returns; NULL: 3.4445, -4.7750,
  * 2.0315 in every step.  They must keep the elements of X, and those of A and b A + c A A off their diagonals, below
  * 100 (operands are fp16 inside; beyond 127 they become infinities).  A schedule that converges stays far below: |X|
- * and |A| below 2, and b A + c A A, which maps a singular value s to p(s) / s - a, below 20.  stride_g, stride_o: elements from one matrix of the stack to
+ * and |A| below 2, and b A + c A A, which maps a singular value s to p(s) / s - a, below 25.  stride_g, stride_o: elements from one matrix of the stack to
  * the next. */
 int rl_orthogonalize(const rl_ortho_config* cfg, const float* coefficients, const void* G, int ldg, long stride_g, void* O,
                      int ldo, long stride_o, void* workspace, size_t workspace_bytes, rl_stream stream);

@@ -72,8 +72,9 @@ int pack(FfnMatrix& m, int rows, int cols, T* space, hipStream_t stream) {
 
 int vec_ok(const void* p, int ld) { return (uintptr_t)p % (4 * ES) == 0 && ld % 4 == 0; }
 
-Store<T> store(void* c, int ldc, int N) {
-  Store<T> s = {};
+template <int SCALED = 0>
+Store<T, SCALED> store(void* c, int ldc, int N) {
+  Store<T, SCALED> s = {};
   s.c[0] = s.c[1] = (T*)c;
   s.ldc = s.ldc1 = ldc;
   s.N = N;
@@ -306,7 +307,7 @@ int backward(const FfnCall& call) {
     Problem p = problem(r.dg, s.pitch, c.w_gate.p, c.w_gate.ld, c.T, c.D, c.F, c.T, c.D);
     p.a[1] = r.du;
     p.b[1] = c.w_up.p;
-    Store<T> out = store(c.dx, c.ld_dx, c.D);
+    auto out = store<is_scaled<T>()>(c.dx, c.ld_dx, c.D);
     out.peaks = r.peaks;
     PT_TRY((run_product<T, 1, 0, 0, 2, 0>(p, r.dx, out, 1, r.pieces, arrivals, c.stream, c.compute_units, "ffn: dx")));
   }
@@ -314,7 +315,7 @@ int backward(const FfnCall& call) {
     PT_TRY(pack(c.x, c.T, c.D, r.x, c.stream));
     Problem p = problem(r.dg, s.pitch, c.x.p, c.x.ld, c.F, c.D, c.T, c.F, c.D);
     p.batch_a = (long)c.T * s.pitch;
-    Store<T> out = store(c.dw_gate, c.ld_dw_gate, c.D);
+    auto out = store<is_scaled<T>()>(c.dw_gate, c.ld_dw_gate, c.D);
     out.c[1] = (T*)c.dw_up;
     out.ldc1 = c.ld_dw_up;
     out.peaks = r.peaks;

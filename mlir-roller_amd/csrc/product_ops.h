@@ -111,13 +111,14 @@ PT_DEV float power_of_peaks(const unsigned* peaks) {
 
 // ---- epilogues --------------------------------------------------------------------------------------
 
-// C = acc, in a caller's matrix: any leading dimension and alignment.
-template <class T>
+// C = acc, in a caller's matrix: any leading dimension and alignment.  SCALED: an operand was held times 2^k, and C is
+// 2^-k acc.
+template <class T, int SCALED = 0>
 struct Store {
   T* c[2];      // one per batch entry
   int ldc, ldc1, N;
   int vec;      // rows of 4 elements are aligned
-  const unsigned* peaks;   // fp16: of the dy by which an operand is scaled, NULL: none is
+  const unsigned* peaks;   // SCALED: of the dy that k is by
   float scale;             // (by at)
   __device__ __forceinline__ Store at(int batch) const {
     Store o = *this;
@@ -125,14 +126,14 @@ struct Store {
       o.c[0] = c[1];
       o.ldc = ldc1;
     }
-    if constexpr (is_scaled<T>()) o.scale = peaks ? power_of_peaks<-1>(peaks) : 1.0f;
+    if constexpr (SCALED) o.scale = power_of_peaks<-1>(peaks);
     return o;
   }
   struct In {};
   __device__ __forceinline__ In get(int, int) const { return {}; }
   __device__ __forceinline__ void put(int m, int n, v4f v, In, bool ok) const {
     if (!ok) return;
-    if constexpr (is_scaled<T>()) v *= scale;
+    if constexpr (SCALED) v *= scale;
     T* to = c[0] + (long)m * ldc + n;
     if (vec && n + 3 < N) {
       store4(to, v);
