@@ -323,7 +323,7 @@ int rl_ffn_forward(const rl_ffn_config* cfg, const void* x, int ldx, const void*
  * NULL, dw_gate and dw_up may both be NULL: not computed.  `saved` is left as it was.  T == 0 writes zeros
  * to the weights' gradients.  The gradients before the gate and up weights are rounded once to dtype on their way;
  * in fp16 they are held times a power of two while every |dy| is below 2^-6, so that small ones keep their bits, and
- * become infinite beyond 65504, or 2^22 times the largest |dy| if that is less. */
+ * become infinite beyond 65504, or beyond 2^21 to 2^22 times the largest |dy| if that is less. */
 int rl_ffn_backward(const rl_ffn_config* cfg, const void* dy, int lddy, const void* x, int ldx, const void* w_gate,
                     int ld_gate, const void* w_up, int ld_up, const void* w_down, int ld_down, const void* saved, void* dx,
                     int lddx, void* dw_gate, int ldd_gate, void* dw_up, int ldd_up, void* dw_down, int ldd_down, int T,

@@ -14,8 +14,8 @@
 //   * bf16 matrices: one fp16 number per operand element, which leaves an error of 0.02 to 0.1 % of the norm,
 //     under the rounding of the output.
 //   * fp16 and fp32 matrices: two, high part and remainder (22 bits), and three of their four products,
-//     hi hi + hi lo + lo hi, as three segments of one K loop: an error of some 10^-7 of the norm, as with fp32
-//     products, at a third of the fp16 rate instead of a sixteenth.
+//     hi hi + hi lo + lo hi, as three segments of one K loop: an error of some 10^-6 of the norm (1.3e-6 at
+//     509 x 1023; fp32 products in the plain form 2.4e-6), at a third of the fp16 rate instead of a sixteenth.
 #include "product_launch.h"
 #include "roller_ortho.h"
 

@@ -47,8 +47,8 @@ PT_DEV float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_am
 
 constexpr float GELU_2C = 1.5957691216f, GELU_C1 = 0.044715f;   // 2 sqrt(2 / pi)
 
-// (1 + erf(g / sqrt 2)) / 2, as erfc of the other sign: 1 + erf has no digits left far below zero (of the activation at -5
-// 3 % were missing, at -6 all of it).
+// (1 + erf(g / sqrt 2)) / 2, as erfc of the other sign: 1 + erf has no digits left far below zero (at -5 the activation
+// would be 4 % off, at -6 zero).
 PT_DEV float normal_below(float g) { return 0.5f * erfcf(-0.70710678f * g); }
 
 template <int KIND>
@@ -83,8 +83,8 @@ PT_DEV void act_slope(float g, float& a, float& slope) {
 // dg and du are operands of two further products and have the element type.  In fp16 a number below 2^-14 has fewer
 // than 11 bits, and that is where the gradients of an unscaled loss are (dy of 1e-6: dW_gate 3 % off).  So they are
 // held times 2^k, and the products made of them leave times 2^-k.  k >= 0 is the least that brings the largest
-// finite |dy| to 2^-6: dg and du around 2^-9 then have all their bits, and they reach infinity at 2^22 times that
-// |dy|.  From |dy| = 2^-6 on k is 0.  (bf16 has the exponents of fp32.)
+// finite |dy| to 2^-6: dg and du around 2^-9 then have all their bits, and they reach infinity at 2^21 to 2^22 times
+// that |dy|.  From |dy| = 2^-6 on k is 0.  (bf16 has the exponents of fp32.)
 
 constexpr int PEAKS = 256;   // workgroups of peak_kernel
 

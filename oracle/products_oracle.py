@@ -190,7 +190,8 @@ def orthogonalise_two_part(G: np.ndarray, steps: int = 5, coefficients=STANDARD,
 
 
 def two_part_excess(got: np.ndarray, exact: np.ndarray, model: np.ndarray, dtype: str) -> float:
-    """How far fp16 or fp32 results are off, in the norm, as a multiple of what they may be.
+    """How far fp16 or fp32 results are off, in the norm, as a multiple of what they may be; for sides of 30 and more,
+    whose many roundings make one sample of an error's norm tell the next one.
 
     ``model`` (orthogonalise_two_part) has the library's roundings and sums of fp32 in another order, one rounding per
     product where a matrix unit has one per 16, so its error e stands for the library's; four times it is allowed, and
